@@ -35,6 +35,7 @@
 #include <string>
 #include <vector>
 
+#include "../kernels/adamw.h"
 #include "../kernels/conv_igemm.h"
 #include "../kernels/conv_wgrad.h"
 #include "../kernels/dense_stage.h"
@@ -95,6 +96,11 @@ enum OpKind : int {
   OP_MB_INFER = 31,
   // a whole DenseNet dense block in inference mode (dense_infer.hip): payload DenseInferArgs
   OP_DENSE_INFER = 32,
+  // multi-tensor AdamW step (adamw.hip): payload AdamwArgs, i[0] state bits, i[1] bf16 gradients
+  OP_ADAMW = 33,
+  // partial sums of the squared gradients (adamw.hip): p[0] device OptChunk[i[0]], p[1] partials,
+  // i[1] bf16 gradients
+  OP_GRAD_NORM = 34,
 };
 
 struct Op {
@@ -453,7 +459,8 @@ class Plan {
                                   "input", "memset", "bn_stats", "bn_apply", "dw_fwd", "dw_bwd_data",
                                   "dw_wgrad", "copy", "finite_check", "mlp_fwd", "mlp_bwd", "mlp_step",
                                   "collapse", "stats_shift", "allreduce", "wgrad_batch", "dense_stage",
-                                  "dense_stage_bwd", "mb_chain", "mb_infer", "dense_infer"};
+                                  "dense_stage_bwd", "mb_chain", "mb_infer", "dense_infer",
+                                  "adamw", "grad_norm"};
     int k = ops_.at(idx).kind;
     return (k >= 0 && k < (int)(sizeof(names) / sizeof(names[0]))) ? names[k] : "?";
   }
@@ -634,6 +641,12 @@ class Plan {
                       reinterpret_cast<float*>(op.p[2]), op.l[0], op.f[0], op.f[1], op.f[2], op.f[3],
                       reinterpret_cast<const int*>(op.p[3]), reinterpret_cast<int*>(op.p[4]), st),
               "rmsprop");
+        break;
+      case OP_ADAMW: check(adamw(as<AdamwArgs>(op), op.i[0], op.i[1], st), "adamw"); break;
+      case OP_GRAD_NORM:
+        check(grad_norm_partials(reinterpret_cast<const OptChunk*>(op.p[0]), op.i[0], op.i[1],
+                                 reinterpret_cast<double*>(op.p[1]), st),
+              "grad_norm");
         break;
       case OP_CAST:
         check(cast_weights(reinterpret_cast<const CastEntry*>(op.p[0]), reinterpret_cast<const int*>(op.p[1]),
@@ -816,6 +829,10 @@ py::dict struct_sizes() {
   d["DenseInferArgs"] = sizeof(DenseInferArgs);
   d["MbChainArgs"] = sizeof(MbChainArgs);
   d["MbPhaseDesc.pre"] = offsetof(MbPhaseDesc, pre);
+  d["OptChunk"] = sizeof(OptChunk);
+  d["AdamwArgs"] = sizeof(AdamwArgs);
+  d["AdamwArgs.log_b1"] = offsetof(AdamwArgs, log_b1);
+  d["AdamwArgs.npartials"] = offsetof(AdamwArgs, npartials);
   d["BnArgs.shift"] = offsetof(BnArgs, shift);
   d["ConvArgs.stats_shift"] = offsetof(ConvArgs, stats_shift);
   d["PoolArgs.stats_shift"] = offsetof(PoolArgs, stats_shift);
@@ -940,6 +957,29 @@ void py_rmsprop(uintptr_t w, uintptr_t g, uintptr_t ms, long long n, float lr, f
   check(rmsprop(reinterpret_cast<float*>(w), reinterpret_cast<const float*>(g), reinterpret_cast<float*>(ms), n,
                 lr, rho, eps, gs, nullptr, nullptr, reinterpret_cast<hipStream_t>(stream)),
         "rmsprop");
+}
+
+// `args`: the address of an AdamwArgs (a ctypes struct of the caller's)
+void py_adamw(uintptr_t args, int bits, int g_bf16, uintptr_t stream) {
+  check(adamw(*reinterpret_cast<const AdamwArgs*>(args), bits, g_bf16, reinterpret_cast<hipStream_t>(stream)), "adamw");
+}
+
+void py_adamw_decode(uintptr_t m, uintptr_t v, uintptr_t scales, long long n, uintptr_t om, uintptr_t ov, int out_bf16,
+                     uintptr_t stream) {
+  check(adamw_decode(reinterpret_cast<const unsigned char*>(m), reinterpret_cast<const unsigned char*>(v),
+                     reinterpret_cast<const unsigned char*>(scales), n, reinterpret_cast<void*>(om),
+                     reinterpret_cast<void*>(ov), out_bf16, reinterpret_cast<hipStream_t>(stream)),
+        "adamw_decode");
+}
+
+// out 0: only the partial sums (the clipping of an AdamW step finishes them)
+void py_grad_norm(uintptr_t chunks, int nchunks, int g_bf16, uintptr_t partials, uintptr_t out, uintptr_t stream) {
+  const OptChunk* c = reinterpret_cast<const OptChunk*>(chunks);
+  double* p = reinterpret_cast<double*>(partials);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  check(out ? grad_norm(c, nchunks, g_bf16, p, reinterpret_cast<float*>(out), st)
+            : grad_norm_partials(c, nchunks, g_bf16, p, st),
+        "grad_norm");
 }
 
 // Pinned host words the device writes and the host polls without a synchronisation (the
@@ -1107,6 +1147,14 @@ PYBIND11_MODULE(_idc_native, m) {
   m.def("tile_bn", &conv_tile_bn);
   m.def("tile_bk", &conv_tile_bk);
   m.def("rmsprop", &py_rmsprop);
+  m.def("adamw", &py_adamw);
+  m.def("adamw_decode", &py_adamw_decode);
+  m.def("grad_norm", &py_grad_norm);
+  m.attr("OPT_CHUNK") = OPT_CHUNK;
+  m.attr("OPT_MAX_GRID") = OPT_MAX_GRID;
+  m.attr("OPT_BLOCK") = OPT_BLOCK;
+  m.attr("OP_ADAMW") = (int)OP_ADAMW;
+  m.attr("OP_GRAD_NORM") = (int)OP_GRAD_NORM;
   m.def("host_alloc", &py_host_alloc);
   m.def("host_free", &py_host_free);
   m.def("secagg_mask", &py_secagg_mask, py::arg("x"), py::arg("out"), py::arg("n"), py::arg("seg_scale"),

@@ -203,6 +203,23 @@ class DenseInferArgs(C.Structure):
                [("layers", vp)]
 
 
+class OptChunk(C.Structure):
+    """One piece of one tensor of a multi-tensor optimizer launch (csrc/kernels/adamw.h)."""
+    _fields_ = [("w", vp), ("g", vp), ("base", cll), ("n", ci), ("flags", ci)]
+
+
+class AdamwArgs(C.Structure):
+    """A multi-tensor AdamW step (csrc/kernels/adamw.h)."""
+    _fields_ = [(n, vp) for n in ("chunks", "m", "v", "scales", "step", "partials", "norm", "skip", "hostflag")] + \
+               [("log_b1", C.c_double), ("log_b2", C.c_double)] + \
+               [(n, cf) for n in ("b1", "omb1", "b2", "omb2", "lr", "eps", "lr_wd", "grad_scale", "clip")] + \
+               [("nchunks", ci), ("npartials", ci)]
+
+
+OPT_CHUNK, OPT_MAX_GRID, OPT_BLOCK = 2048, 1024, 64  # csrc/kernels/adamw.h
+OPT_DECAY, OPT_VEC = 1, 2
+
+
 def mb_infer_default_cs(cexp: int, groups: int, expand: bool = True) -> int:
     """Expanded channels per workgroup of an mb_infer launch (csrc/kernels/mb_infer.h): enough
     slices per image group that the launch has >= 256 workgroups, in multiples of 32."""
@@ -221,7 +238,7 @@ _STRUCTS = {"BnArgs": BnArgs, "BwdAff": BwdAff, "ConvArgs": ConvArgs, "WgradArgs
             "DenseStageArgs": DenseStageArgs, "DenseLayerDesc": DenseLayerDesc,
             "DenseBwdArgs": DenseBwdArgs, "DenseBwdLayerDesc": DenseBwdLayerDesc, "DenseBwdPhase": DenseBwdPhase,
             "MbPhaseDesc": MbPhaseDesc, "MbChainArgs": MbChainArgs, "MbInferArgs": MbInferArgs,
-            "DenseInferArgs": DenseInferArgs}
+            "DenseInferArgs": DenseInferArgs, "OptChunk": OptChunk, "AdamwArgs": AdamwArgs}
 
 # op kinds (csrc/runtime/plan.cpp)
 OP_CONV, OP_WGRAD, OP_BN_BWD_APPLY, OP_BN_BWD_REDUCE, OP_MAXPOOL, OP_AVGPOOL, OP_POOL_BWD = range(7)
@@ -233,6 +250,7 @@ OP_DENSE_STAGE_BWD = 29
 OP_MB_CHAIN = 30
 OP_MB_INFER = 31
 OP_DENSE_INFER = 32
+OP_ADAMW, OP_GRAD_NORM = 33, 34
 
 ACT = {None: 0, "none": 0, "linear": 0, "relu": 1, "relu6": 2}
 OUT_BF16, OUT_F32, OUT_F32_ACC = 0, 1, 2
@@ -244,6 +262,9 @@ def _verify(ext):
     if ext.OP_DENSE_STAGE != OP_DENSE_STAGE or ext.OP_MB_CHAIN != OP_MB_CHAIN or ext.OP_MB_INFER != OP_MB_INFER \
             or ext.OP_DENSE_INFER != OP_DENSE_INFER:
         raise RuntimeError("native op-kind table drifted (OP_DENSE_STAGE / OP_MB_CHAIN)")
+    if (ext.OP_ADAMW, ext.OP_GRAD_NORM) != (OP_ADAMW, OP_GRAD_NORM) \
+            or (ext.OPT_CHUNK, ext.OPT_MAX_GRID, ext.OPT_BLOCK) != (OPT_CHUNK, OPT_MAX_GRID, OPT_BLOCK):
+        raise RuntimeError("native multi-tensor optimizer constants drifted")
     sizes = ext.struct_sizes()
     for name, cls in _STRUCTS.items():
         if C.sizeof(cls) != sizes[name]:
@@ -262,7 +283,8 @@ def _verify(ext):
               "ConvArgs.stats_shift": ConvArgs.stats_shift.offset,
               "PoolArgs.stats_shift": PoolArgs.stats_shift.offset,
               "DwArgs.stats_shift": DwArgs.stats_shift.offset,
-              "BnMovingDesc.shift": BnMovingDesc.shift.offset, "MbPhaseDesc.pre": MbPhaseDesc.pre.offset}
+              "BnMovingDesc.shift": BnMovingDesc.shift.offset, "MbPhaseDesc.pre": MbPhaseDesc.pre.offset,
+              "AdamwArgs.log_b1": AdamwArgs.log_b1.offset, "AdamwArgs.npartials": AdamwArgs.npartials.offset}
     for k, v in checks.items():
         if sizes[k] != v:
             raise RuntimeError(f"native struct field {k}: ctypes offset {v} != C++ {sizes[k]}")

@@ -49,6 +49,7 @@ SOURCES = [
     "kernels/dense_rows_bwd.hip",
     "kernels/mlp_head.hip",
     "kernels/secagg.hip",
+    "kernels/adamw.hip",
     "comm/communicator.cpp",
     "runtime/plan.cpp",
     "runtime/guard_alloc.cpp",
