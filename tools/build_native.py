@@ -83,7 +83,11 @@ def _compile(src: str, extra) -> str:
         return o
     cmd = [HIPCC, f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-c", s, "-o", o,
            f"-I{pybind11.get_include()}", f"-I{sysconfig.get_paths()['include']}",
-           "-Wno-unused-result", "-Wno-unused-variable"]
+           "-Wno-unused-result", "-Wno-unused-variable",
+           # no packed fp32 arithmetic (v_pk_mul_f32 and its like, which -O3 forms by itself): some of
+           # its forms have given wrong results on these machines.  The host pass does not know the
+           # feature and says so.
+           "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
     # MFMA accumulators in the VGPR form: without it the register allocator keeps them in AGPRs ON
     # TOP of the kernel's VGPRs (unified register file), one occupancy step below what the kernel
     # needs -- e.g. the DenseNet concat-gradient dgrad tile 126 VGPRs + 16 AGPRs = 3 waves/SIMD,
