@@ -8,10 +8,14 @@ struct OptChunk {
   float* w;          // weights of the piece (null in a table that only serves the norm)
   const void* g;     // gradients, fp32 or bf16
   long long base;    // the piece's place in the flat state: a multiple of 64
-  int n;             // elements, 1 .. OPT_CHUNK
+  int n;             // elements, 1 .. the table's chunk size
   int flags;         // bit 0: weight decay; bit 1: w and g may be read and written as vectors of 4
 };
-constexpr int OPT_CHUNK = 2048;       // elements a workgroup takes at a time
+// Elements a workgroup takes at a time: OPT_CHUNK, and OPT_CHUNK_BIG in a table that has at least
+// OPT_MAX_GRID pieces of that size.  us for fp32 gradients, 32-bit states, 2048 / 4096: 2.2M weights 11.4 /
+// 11.8, 7M 36.0 / 35.8, 40M 225 / 216, 120M 669 / 655.
+constexpr int OPT_CHUNK = 2048, OPT_CHUNK_BIG = 4096;
+constexpr long long OPT_NT_BYTES = 128ll << 20;  // what is read and written from here on goes past the caches
 constexpr int OPT_MAX_GRID = 1024;    // workgroups of a launch, copies of the step counter, partial sums
 constexpr int OPT_NORM_ONE = 8;       // chunks that one workgroup sums by itself (grad_norm)
 constexpr int OPT_DECAY = 1, OPT_VEC = 2;
@@ -23,15 +27,17 @@ struct AdamwArgs {
   void* v;                  // second moments: fp32, or 8-bit codes of their roots
   unsigned char* scales;    // 8-bit states: [block][2] scale bytes (first moment, root)
   int* step;                // [OPT_MAX_GRID] copies of the steps done
-  const double* partials;   // sums of squared gradients (grad_norm_partials), null: no clipping
-  float* norm;              // the global norm, written when there is clipping
+  const double* partials;   // sums of squared gradients (grad_norm_partials); null with clipping: at
+                            // most OPT_NORM_ONE pieces, the step sums them itself
+  float* norm;              // [4] the global norm, written when there is clipping; work space
   const int* skip;          // nullable guard word: not zero = this step changes nothing
   int* hostflag;            // nullable pinned host word (rmsprop's)
   double log_b1, log_b2;    // natural logarithms of beta_1, beta_2 (-inf for 0)
   float b1, omb1, b2, omb2; // betas, and 1 - beta rounded from double
   float lr, eps, lr_wd;     // lr_wd = learning rate * weight decay
-  float grad_scale, clip;   // clip: largest norm of the scaled gradients
+  float grad_scale, clip;   // clip: largest norm of the scaled gradients (0: no clipping)
   int nchunks, npartials;
+  int chunk, pad;           // the table's chunk size
 };
 
 inline int opt_grid(int nchunks) { return nchunks < 1 ? 1 : nchunks > OPT_MAX_GRID ? OPT_MAX_GRID : nchunks; }

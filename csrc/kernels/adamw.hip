@@ -10,7 +10,8 @@
 //
 // The step counter is OPT_MAX_GRID equal words: a workgroup reads its own and writes it (and those
 // of the workgroups this launch does not have) at its end, so a captured launch counts its replays
-// without an atomic, a second launch, or a word that one workgroup writes while another reads it.
+// without an atomic, a second launch, or a word that one workgroup writes while another reads it.  (The
+// largest tables have a launch of one workgroup ahead that counts: adamw_begin_kernel.)
 //
 // 8-bit states.  64 neighbouring elements of a tensor share two scale bytes, one for m and one for
 // r = sqrt(v); a scale byte s is the unit 2^(s-127) of the block's codes, the smallest one with which
@@ -30,28 +31,42 @@ namespace idc {
 
 namespace {
 
-constexpr int TPB = 256;                         // threads of a workgroup
-constexpr int ROWS = OPT_CHUNK / (TPB * 4);      // groups of 4 elements a thread takes of a chunk
+constexpr int TPB = 256;  // threads of a workgroup; a row is the TPB * 4 elements they take at once
 
 struct F4 {
   float a[4];
 };
+typedef float vf4 __attribute__((ext_vector_type(4)));
 
+// NT: past the caches (see `adamw`)
+template <bool NT = false, typename T>
+__device__ __forceinline__ T ld(const T* p) {
+  if constexpr (NT) return __builtin_nontemporal_load(p);
+  else return *p;
+}
+template <bool NT = false, typename T>
+__device__ __forceinline__ void st(T* p, T x) {
+  if constexpr (NT) __builtin_nontemporal_store(x, p);
+  else *p = x;
+}
+template <bool NT = false>
 __device__ __forceinline__ F4 ld4(const float* p) {
-  const float4 x = *reinterpret_cast<const float4*>(p);
+  const vf4 x = ld<NT>(reinterpret_cast<const vf4*>(p));
   return F4{{x.x, x.y, x.z, x.w}};
 }
+template <bool NT = false>
 __device__ __forceinline__ void st4(float* p, const F4& x) {
-  *reinterpret_cast<float4*>(p) = make_float4(x.a[0], x.a[1], x.a[2], x.a[3]);
+  st<NT>(reinterpret_cast<vf4*>(p), vf4{x.a[0], x.a[1], x.a[2], x.a[3]});
 }
-template <bool GB>
+template <bool GB, bool NT = false>
 __device__ __forceinline__ F4 ldg4(const void* g, int e) {
   if constexpr (GB) {
-    const uint2 x = *reinterpret_cast<const uint2*>(reinterpret_cast<const bf16_t*>(g) + e);
+    typedef unsigned vu2 __attribute__((ext_vector_type(2)));
+    const vu2 x = ld<NT>(reinterpret_cast<const vu2*>(reinterpret_cast<const bf16_t*>(g) + e));
     return F4{{__uint_as_float(x.x << 16), __uint_as_float(x.x & 0xffff0000u), __uint_as_float(x.y << 16),
                __uint_as_float(x.y & 0xffff0000u)}};
   } else {
-    return ld4(reinterpret_cast<const float*>(g) + e);
+    return ld4<NT>(reinterpret_cast<const float*>(g) + e);
   }
 }
 template <bool GB>
@@ -108,25 +123,39 @@ __device__ __forceinline__ double block_sum64(double v) {
 }
 
 // --- the codes ------------------------------------------------------------------------------
-// MB mantissa bits: a code shifted by 23 - MB is a float's bits; its unit is that float's 2^-(126+MB)
+// A code of MB mantissa bits, its bits at a float's place (shifted by 23 - MB), times 2^(126+MB) is
+// its value in units; the unit is 2^(s-127).
 template <int MB>
-__device__ __forceinline__ float code_value(unsigned c, int s) {
-  return ldexpf(__uint_as_float(c << (23 - MB)), s - 127 + 126 + MB);
+__device__ __forceinline__ float code_value(unsigned x, int s) {
+  return ldexpf(__uint_as_float(x), s - 127 + 126 + MB);
+}
+// byte j of a word of first moments (sign and 7 bits), and of a word of roots
+template <int J>
+__device__ __forceinline__ float m_value(unsigned word, int s) {
+  return code_value<3>((unsigned)((int)(word << (24 - 8 * J)) >> 4) & 0x87f00000u, s);
+}
+template <int J>
+__device__ __forceinline__ float root_value(unsigned word, int s) {
+  return code_value<4>((word >> (8 * J) & 255u) << 19, s);
 }
 
 // scale byte for a block whose largest magnitude has these bits: codes reach (2^(MB+1) - 1) * 2^14
 template <int MB>
 __device__ __forceinline__ int block_scale(unsigned top) {
-  constexpr unsigned last = ((2u << MB) - 1u) << (23 - MB) & 0x7fffffu;  // mantissa of the largest code
+  constexpr unsigned last = (((2u << MB) - 1u) << (23 - MB)) & 0x7fffffu;  // mantissa of the largest code
   const int s = (int)((top + (0x7fffffu - last)) >> 23) - (14 + MB);
   return top >= 0x7f800000u ? 255 : s < 1 ? 1 : s;
 }
 
-// magnitude code of a (>= 0) with 16 random bits; a <= the block's largest
+// the code of |a| <= the block's largest, in the bits from 23 - MB on (what is below is left over);
+// bits: 16 random ones, in the bits from 7 - MB on, and the half of the last of them
 template <int MB>
-__device__ __forceinline__ unsigned code_of(float a, int s, unsigned r16) {
-  const unsigned x = __float_as_uint(ldexpf(a, -(s - 127 + 126 + MB)));
-  return (x + (r16 << (7 - MB)) + (1u << (6 - MB))) >> (23 - MB);
+__device__ __forceinline__ unsigned code_of(float a, int s, unsigned bits) {
+  return __float_as_uint(ldexpf(fabsf(a), -(s - 127 + 126 + MB))) + bits;
+}
+
+__device__ __forceinline__ unsigned top_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0c0c0703u), __builtin_amdgcn_perm(b, a, 0x0c0c0703u), 0x05040100u);
 }
 
 // largest of the 16 lanes that hold a block
@@ -164,20 +193,23 @@ __device__ __forceinline__ void moments(F4& m, F4& v, const F4& g, float b1, flo
     v.a[j] = b2 * v.a[j] + h.omb2 * (x * x);
   }
 }
-// the decay is subtracted, not multiplied as (1 - lr wd): that factor would keep few of lr wd's bits
+// The decay is subtracted, not multiplied as (1 - lr wd): that factor would keep few of lr wd's bits.
+// The quotient is a reciprocal (to one unit in its last place) and a product: 3 half steps of fp32 in
+// the update, which a weight's own rounding hides, for a third of a division's instructions.
 __device__ __forceinline__ void update(F4& w, const F4& m, const F4& root, float lr_wd, const Hyper& h) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) w.a[j] -= fmaf(lr_wd, w.a[j], h.alpha * (m.a[j] / (root.a[j] + h.eps)));
+  for (int j = 0; j < 4; ++j)
+    w.a[j] -= fmaf(lr_wd, w.a[j], h.alpha * (m.a[j] * __builtin_amdgcn_rcpf(root.a[j] + h.eps)));
 }
 
-template <int BITS>
+template <int BITS, bool NT>
 struct State;
-template <>
-struct State<32> {
+template <bool NT>
+struct State<32, NT> {
   F4 m, v;
   __device__ __forceinline__ void load(const AdamwArgs& a, long long i) {
-    m = ld4(reinterpret_cast<const float*>(a.m) + i);
-    v = ld4(reinterpret_cast<const float*>(a.v) + i);
+    m = ld4<NT>(reinterpret_cast<const float*>(a.m) + i);
+    v = ld4<NT>(reinterpret_cast<const float*>(a.v) + i);
   }
   __device__ __forceinline__ void step(const AdamwArgs& a, long long i, F4& w, const F4& g, float lr_wd,
                                        const Hyper& h, unsigned) {
@@ -186,31 +218,28 @@ struct State<32> {
 #pragma unroll
     for (int j = 0; j < 4; ++j) root.a[j] = sqrtf(v.a[j]);
     update(w, m, root, lr_wd, h);
-    st4(reinterpret_cast<float*>(a.m) + i, m);
-    st4(reinterpret_cast<float*>(a.v) + i, v);
+    st4<NT>(reinterpret_cast<float*>(a.m) + i, m);
+    st4<NT>(reinterpret_cast<float*>(a.v) + i, v);
   }
 };
-template <>
-struct State<8> {
+template <bool NT>
+struct State<8, NT> {
   unsigned m4, v4;
   unsigned short sc;
   __device__ __forceinline__ void load(const AdamwArgs& a, long long i) {
-    m4 = *reinterpret_cast<const unsigned*>(reinterpret_cast<const unsigned char*>(a.m) + i);
-    v4 = *reinterpret_cast<const unsigned*>(reinterpret_cast<const unsigned char*>(a.v) + i);
+    m4 = ld<NT>(reinterpret_cast<const unsigned*>(reinterpret_cast<const unsigned char*>(a.m) + i));
+    v4 = ld<NT>(reinterpret_cast<const unsigned*>(reinterpret_cast<const unsigned char*>(a.v) + i));
     sc = reinterpret_cast<const unsigned short*>(a.scales)[i / OPT_BLOCK];
   }
   __device__ __forceinline__ void step(const AdamwArgs& a, long long i, F4& w, const F4& g, float lr_wd,
                                        const Hyper& h, unsigned salt) {
     const int sm = sc & 255, sv = sc >> 8;
-    F4 m, v, root;
+    F4 m = {{m_value<0>(m4, sm), m_value<1>(m4, sm), m_value<2>(m4, sm), m_value<3>(m4, sm)}};
+    F4 root = {{root_value<0>(v4, sv), root_value<1>(v4, sv), root_value<2>(v4, sv), root_value<3>(v4, sv)}};
+    F4 v;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const unsigned cm = (m4 >> (8 * j)) & 255u, cv = (v4 >> (8 * j)) & 255u;
-      m.a[j] = __uint_as_float(__float_as_uint(code_value<3>(cm & 127u, sm)) | ((cm & 128u) << 24));
-      const float r = code_value<4>(cv, sv);
-      v.a[j] = r * r;
-    }
-    // a block that holds no finite moment reads as NaN: through its factor
+    for (int j = 0; j < 4; ++j) v.a[j] = root.a[j] * root.a[j];
+    // a block that holds a moment that is not finite reads as NaN: through its factor
     const float nan = __uint_as_float(0x7fc00000u);
     moments(m, v, g, sm == 255 ? nan : h.b1, sv == 255 ? nan : h.b2, h);
     unsigned tm = 0, tv = 0;
@@ -223,25 +252,27 @@ struct State<8> {
     update(w, m, root, lr_wd, h);
     const int nm = block_scale<3>(max16(tm)), nv = block_scale<4>(max16(tv));
     const unsigned place = (unsigned)i + (unsigned)(i >> 32) * HASH_HIGH + salt;
-    unsigned om = 0, ov = 0;
+    unsigned c[4], d[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const unsigned r = dither(place + j);
-      const unsigned c = code_of<3>(fabsf(m.a[j]), nm, r & 0xffffu) | ((__float_as_uint(m.a[j]) >> 24) & 128u);
-      const unsigned d = max(code_of<4>(root.a[j], nv, r >> 16), root.a[j] > 0.f ? 1u : 0u);
-      om |= c << (8 * j);
-      ov |= d << (8 * j);
+      // codes to the top byte of a word: the sign over 7 bits, or 8 bits
+      c[j] = (code_of<3>(m.a[j], nm, (r << 16 | 0x8000u) >> 12) << 4 & 0x7fffffffu) | (__float_as_uint(m.a[j]) & 0x80000000u);
+      d[j] = max(code_of<4>(root.a[j], nv, (r >> 13 & 0x7fff8u) | 4u) << 5, min(__float_as_uint(root.a[j]), 1u << 24));
     }
-    *reinterpret_cast<unsigned*>(reinterpret_cast<unsigned char*>(a.m) + i) = nm == 255 ? 0u : om;
-    *reinterpret_cast<unsigned*>(reinterpret_cast<unsigned char*>(a.v) + i) = nv == 255 ? 0u : ov;
+    const unsigned om = nm == 255 ? 0u : top_bytes(c[0], c[1], c[2], c[3]);
+    const unsigned ov = nv == 255 ? 0u : top_bytes(d[0], d[1], d[2], d[3]);
+    st<NT>(reinterpret_cast<unsigned*>(reinterpret_cast<unsigned char*>(a.m) + i), om);
+    st<NT>(reinterpret_cast<unsigned*>(reinterpret_cast<unsigned char*>(a.v) + i), ov);
     if ((threadIdx.x & 15) == 0)
       reinterpret_cast<unsigned short*>(a.scales)[i / OPT_BLOCK] = (unsigned short)(nm | (nv << 8));
   }
 };
 
-template <int BITS, bool GB>
-__global__ __launch_bounds__(TPB) void adamw_kernel(AdamwArgs a, GroupArg ga) {
-  const long long go = goff(ga);
+template <bool GB>
+__device__ __forceinline__ double chunk_squares(const OptChunk& k);
+
+__device__ __forceinline__ AdamwArgs shifted(AdamwArgs a, long long go) {
   a.chunks = gsh(a.chunks, go);
   a.m = gsh(reinterpret_cast<char*>(a.m), go);
   a.v = gsh(reinterpret_cast<char*>(a.v), go);
@@ -250,23 +281,75 @@ __global__ __launch_bounds__(TPB) void adamw_kernel(AdamwArgs a, GroupArg ga) {
   a.partials = gsh(a.partials, go);
   a.norm = gsh(a.norm, go);
   a.skip = gsh(a.skip, go);
+  return a;
+}
+// lr sqrt(1 - b2^t) / (1 - b1^t);  1 - b^t = -expm1(t log b): the product in double, so that its
+// rounding does not grow with t
+__device__ __forceinline__ float alpha_of(const AdamwArgs& a, int t) {
+  return a.lr * sqrtf(-expm1f((float)(t * a.log_b2))) / -expm1f((float)(t * a.log_b1));
+}
+// factor of the scaled gradients; a norm that is not finite makes every gradient NaN
+__device__ __forceinline__ float clip_of(const AdamwArgs& a, float norm) {
+  const float scaled = norm * fabsf(a.grad_scale);
+  return scaled <= a.clip ? 1.f : scaled < INFINITY ? a.clip / scaled : __uint_as_float(0x7fc00000u);
+}
+__device__ __forceinline__ float norm_of(const double* partials, int n) {
+  double s = 0.0;
+  for (int i = threadIdx.x; i < n; i += TPB) s += partials[i];
+  return (float)sqrt(block_sum64(s));
+}
+
+// What a launch of one workgroup a piece (FULL) reads instead of working it out in each of them:
+// counts the step and leaves norm, alpha, the gradients' factor and the step's number.
+__global__ __launch_bounds__(TPB) void adamw_begin_kernel(AdamwArgs a, GroupArg ga) {
+  a = shifted(a, goff(ga));
+  if (a.skip && *a.skip) return;
+  const int t = a.step[0] + 1;
+  float norm = 0.f, clip = 1.f;
+  if (a.clip > 0.f) {
+    norm = norm_of(a.partials, a.npartials);
+    clip = clip_of(a, norm);
+  }
+  __syncthreads();  // every wave has read the counter
+  for (int i = threadIdx.x; i < OPT_MAX_GRID; i += TPB) a.step[i] = t;
+  if (threadIdx.x == 0) {
+    if (a.clip > 0.f) a.norm[0] = norm;
+    a.norm[1] = alpha_of(a, t);
+    a.norm[2] = clip;
+    a.norm[3] = __int_as_float(t);
+  }
+}
+
+template <int BITS, bool GB, int ROWS, bool NT, bool FULL>
+__global__ __launch_bounds__(TPB) void adamw_kernel(AdamwArgs a, GroupArg ga) {
+  const long long go = goff(ga);
+  a = shifted(a, go);
   if (a.skip && *a.skip) {  // moments, weights and the step counter stay as they are
     if (a.hostflag && (*a.skip & ~1) && blockIdx.x == 0 && threadIdx.x == 0)  // as rmsprop_kernel
       __hip_atomic_store(a.hostflag, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_SYSTEM);
     return;
   }
-  const int t = a.step[blockIdx.x] + 1;
+  int t;
   Hyper h{a.b1, a.omb1, a.b2, a.omb2, 0.f, a.eps, a.grad_scale, 1.f};
-  // 1 - b^t = -expm1(t log b): the product in double, so that its rounding does not grow with t
-  h.alpha = a.lr * sqrtf(-expm1f((float)(t * a.log_b2))) / -expm1f((float)(t * a.log_b1));
-  if (a.partials) {
-    double s = 0.0;
-    for (int i = threadIdx.x; i < a.npartials; i += TPB) s += a.partials[i];
-    const float norm = (float)sqrt(block_sum64(s));
-    if (blockIdx.x == 0 && threadIdx.x == 0) *a.norm = norm;
-    const float scaled = norm * fabsf(a.grad_scale);
-    // a norm that is not finite makes every gradient NaN
-    h.clip = scaled <= a.clip ? 1.f : scaled < INFINITY ? a.clip / scaled : __uint_as_float(0x7fc00000u);
+  if constexpr (FULL) {
+    h.alpha = a.norm[1];
+    h.clip = a.norm[2];
+    t = __float_as_int(a.norm[3]);
+  } else {
+    t = a.step[blockIdx.x] + 1;
+    h.alpha = alpha_of(a, t);
+    if (a.clip > 0.f) {
+      float norm;
+      if (a.partials) {
+        norm = norm_of(a.partials, a.npartials);
+      } else {  // a small table: every workgroup sums all of it
+        double s = 0.0;
+        for (int c = 0; c < a.nchunks; ++c) s += chunk_squares<GB>(get_chunk(a.chunks + c, go));
+        norm = (float)sqrt(block_sum64(s));
+      }
+      if (blockIdx.x == 0 && threadIdx.x == 0) a.norm[0] = norm;
+      h.clip = clip_of(a, norm);
+    }
   }
   const unsigned salt = (unsigned)t * HASH_STEP;
   const int e0 = threadIdx.x * 4;
@@ -274,66 +357,89 @@ __global__ __launch_bounds__(TPB) void adamw_kernel(AdamwArgs a, GroupArg ga) {
     const OptChunk k = get_chunk(a.chunks + c, go);
     const float lr_wd = k.flags & OPT_DECAY ? a.lr_wd : 0.f;
     const bool vec = k.flags & OPT_VEC;
-    State<BITS> s[ROWS];
+    State<BITS, NT> s[ROWS];
     F4 w[ROWS], g[ROWS];
-    if (vec && k.n == OPT_CHUNK) {
+    if (vec && k.n == ROWS * TPB * 4) {
 #pragma unroll
       for (int u = 0; u < ROWS; ++u) {
         const int e = e0 + u * TPB * 4;
-        w[u] = ld4(k.w + e);
-        g[u] = ldg4<GB>(k.g, e);
+        w[u] = ld4<NT>(k.w + e);
+        g[u] = ldg4<GB, FULL && !GB>(k.g, e);
         s[u].load(a, k.base + e);
       }
 #pragma unroll
       for (int u = 0; u < ROWS; ++u) {
         const int e = e0 + u * TPB * 4;
         s[u].step(a, k.base + e, w[u], g[u], lr_wd, h, salt);
-        st4(k.w + e, w[u]);
+        st4<NT>(k.w + e, w[u]);
       }
     } else {
       // the state reaches to the next multiple of 64, so whole blocks (16 lanes) take part
       const int end = (k.n + OPT_BLOCK - 1) / OPT_BLOCK * OPT_BLOCK;
-#pragma unroll
-      for (int u = 0; u < ROWS; ++u) {
-        const int e = e0 + u * TPB * 4;
-        if (e < end) {
-          w[u] = edge_w(k.w, e, k.n, vec);
-          g[u] = edge_g<GB>(k.g, e, k.n, vec);
-          s[u].load(a, k.base + e);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < ROWS; ++u) {
-        const int e = e0 + u * TPB * 4;
-        if (e < end) {
-          s[u].step(a, k.base + e, w[u], g[u], lr_wd, h, salt);
-          edge_st(k.w, e, k.n, vec, w[u]);
-        }
+      for (int e = e0; e < end; e += TPB * 4) {
+        w[0] = edge_w(k.w, e, k.n, vec);
+        g[0] = edge_g<GB>(k.g, e, k.n, vec);
+        s[0].load(a, k.base + e);
+        s[0].step(a, k.base + e, w[0], g[0], lr_wd, h, salt);
+        edge_st(k.w, e, k.n, vec, w[0]);
       }
     }
   }
-  __syncthreads();  // every wave has read the counter
-  for (int i = blockIdx.x + threadIdx.x * gridDim.x; i < OPT_MAX_GRID; i += TPB * gridDim.x) a.step[i] = t;
+  if constexpr (!FULL) {
+    __syncthreads();  // every wave has read the counter
+    for (int i = blockIdx.x + threadIdx.x * gridDim.x; i < OPT_MAX_GRID; i += TPB * gridDim.x) a.step[i] = t;
+  }
 }
 
-// Squares and sums in double: gradients below 1e-19 or above 1e19 have no fp32 squares, and the
-// double units keep up with memory.  Each workgroup sums its pieces in a fixed order.
-template <bool GB>
-__device__ __forceinline__ double chunk_squares(const OptChunk& k, int e0) {
-  double s[4] = {0.0, 0.0, 0.0, 0.0};
-  const bool vec = k.flags & OPT_VEC;
-  F4 g[ROWS];
+// Squares and sums in double: gradients below 1e-19 or above 1e19 have no fp32 squares.  Each
+// workgroup sums its pieces in a fixed order.
+__device__ __forceinline__ double sum4(const F4& g) {
+  double s = 0.0;
 #pragma unroll
-  for (int u = 0; u < ROWS; ++u) {
-    const int e = e0 + u * TPB * 4;
-    if (vec && k.n == OPT_CHUNK) g[u] = ldg4<GB>(k.g, e);
-    else g[u] = edge_g<GB>(k.g, e, k.n, vec);
+  for (int j = 0; j < 4; ++j) s = fma((double)g.a[j], (double)g.a[j], s);
+  return s;
+}
+// this thread's part of a full piece's sum
+template <bool GB, int ROWS>
+__device__ __forceinline__ double full_squares(const OptChunk& k) {
+  double s = 0.0;
+  if constexpr (GB) {
+    // Converting to double costs more than reading a bf16 (120M: 72 us against 60).  Its square is
+    // exact in fp32, so a thread's squares of this piece are summed there, unless their sum is so small or
+    // large that some may have left fp32's range.
+    uint4 x[ROWS / 2];
+#pragma unroll
+    for (int u = 0; u < ROWS / 2; ++u)
+      x[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const bf16_t*>(k.g) + threadIdx.x * 8 + u * TPB * 8);
+    float f[ROWS / 2][8], q = 0.f;
+#pragma unroll
+    for (int u = 0; u < ROWS / 2; ++u) {
+      unpack8(x[u], f[u]);
+      q += ((f[u][0] * f[u][0] + f[u][1] * f[u][1]) + (f[u][2] * f[u][2] + f[u][3] * f[u][3])) +
+           ((f[u][4] * f[u][4] + f[u][5] * f[u][5]) + (f[u][6] * f[u][6] + f[u][7] * f[u][7]));
+    }
+    if (q > 0x1p-90f && q < 0x1p100f) return (double)q;
+#pragma unroll
+    for (int u = 0; u < ROWS / 2; ++u)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s = fma((double)f[u][j], (double)f[u][j], s);
+  } else {
+    F4 g[ROWS];
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u) g[u] = ldg4<GB>(k.g, threadIdx.x * 4 + u * TPB * 4);
+#pragma unroll
+    for (int u = 0; u < ROWS; ++u) s += sum4(g[u]);
   }
-#pragma unroll
-  for (int u = 0; u < ROWS; ++u)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) s[j] = fma((double)g[u].a[j], (double)g[u].a[j], s[j]);
-  return (s[0] + s[1]) + (s[2] + s[3]);
+  return s;
+}
+template <bool GB>
+__device__ __forceinline__ double chunk_squares(const OptChunk& k) {
+  const bool vec = k.flags & OPT_VEC;
+  if (vec && k.n == OPT_CHUNK_BIG) return full_squares<GB, OPT_CHUNK_BIG / (TPB * 4)>(k);
+  if (vec && k.n == OPT_CHUNK) return full_squares<GB, OPT_CHUNK / (TPB * 4)>(k);
+  double s = 0.0;
+  for (int e = threadIdx.x * 4; e < k.n; e += TPB * 4) s += sum4(edge_g<GB>(k.g, e, k.n, vec));
+  return s;
 }
 
 template <bool GB, bool LAST>
@@ -344,8 +450,7 @@ __global__ __launch_bounds__(TPB) void grad_norm_kernel(const OptChunk* chunks, 
   partials = gsh(partials, go);
   out = gsh(out, go);
   double s = 0.0;
-  for (int c = blockIdx.x; c < nchunks; c += gridDim.x)
-    s += chunk_squares<GB>(get_chunk(chunks + c, go), threadIdx.x * 4);
+  for (int c = blockIdx.x; c < nchunks; c += gridDim.x) s += chunk_squares<GB>(get_chunk(chunks + c, go));
   s = block_sum64(s);
   if (threadIdx.x == 0) {
     if (LAST) *out = (float)sqrt(s);
@@ -354,53 +459,87 @@ __global__ __launch_bounds__(TPB) void grad_norm_kernel(const OptChunk* chunks, 
 }
 
 __global__ __launch_bounds__(TPB) void norm_of_partials_kernel(const double* partials, int n, float* out) {
-  double s = 0.0;
-  for (int i = threadIdx.x; i < n; i += TPB) s += partials[i];
-  s = block_sum64(s);
-  if (threadIdx.x == 0) *out = (float)sqrt(s);
+  const float norm = norm_of(partials, n);
+  if (threadIdx.x == 0) *out = norm;
 }
 
-template <bool OB>
+// A thread takes 8 codes of each kind: in bf16 their values are one 16-byte store.
+template <bool OB, bool NT>
 __global__ __launch_bounds__(TPB) void adamw_decode_kernel(const unsigned char* m, const unsigned char* v,
-                                                           const unsigned char* scales, long long n4, void* om,
+                                                           const unsigned char* scales, long long n8, void* om,
                                                            void* ov) {
-  for (long long i = blockIdx.x * (long long)TPB + threadIdx.x; i < n4; i += (long long)gridDim.x * TPB) {
-    const unsigned m4 = reinterpret_cast<const unsigned*>(m)[i], v4 = reinterpret_cast<const unsigned*>(v)[i];
-    const unsigned sc = reinterpret_cast<const unsigned short*>(scales)[i / (OPT_BLOCK / 4)];
+  typedef unsigned vu2 __attribute__((ext_vector_type(2)));
+  typedef unsigned vu4 __attribute__((ext_vector_type(4)));
+  const long long i = blockIdx.x * (long long)TPB + threadIdx.x;
+  if (i < n8) {
+    const vu2 m8 = ld<NT>(reinterpret_cast<const vu2*>(m) + i), v8 = ld<NT>(reinterpret_cast<const vu2*>(v) + i);
+    const unsigned sc = reinterpret_cast<const unsigned short*>(scales)[i / (OPT_BLOCK / 8)];
     const int sm = sc & 255, sv = sc >> 8;
     const float nan = __uint_as_float(0x7fc00000u);
-    F4 x, y;
+    F4 x[2], y[2];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const unsigned cm = (m4 >> (8 * j)) & 255u, cv = (v4 >> (8 * j)) & 255u;
-      const float f = code_value<3>(cm & 127u, sm);
-      x.a[j] = sm == 255 ? nan : cm & 128u ? -f : f;
-      y.a[j] = sv == 255 ? nan : code_value<4>(cv, sv);
+    for (int k = 0; k < 2; ++k) {
+      x[k] = F4{{m_value<0>(m8[k], sm), m_value<1>(m8[k], sm), m_value<2>(m8[k], sm), m_value<3>(m8[k], sm)}};
+      y[k] = F4{{root_value<0>(v8[k], sv), root_value<1>(v8[k], sv), root_value<2>(v8[k], sv), root_value<3>(v8[k], sv)}};
+      if (sm == 255) x[k] = F4{{nan, nan, nan, nan}};
+      if (sv == 255) y[k] = F4{{nan, nan, nan, nan}};
     }
-    if (OB) {  // exact: at most 5 significant bits
-      reinterpret_cast<uint2*>(om)[i] = make_uint2(pack2bf(x.a[0], x.a[1]), pack2bf(x.a[2], x.a[3]));
-      reinterpret_cast<uint2*>(ov)[i] = make_uint2(pack2bf(y.a[0], y.a[1]), pack2bf(y.a[2], y.a[3]));
+    if constexpr (OB) {  // exact: at most 5 significant bits
+      st<NT>(reinterpret_cast<vu4*>(om) + i, vu4{pack2bf(x[0].a[0], x[0].a[1]), pack2bf(x[0].a[2], x[0].a[3]),
+                                                 pack2bf(x[1].a[0], x[1].a[1]), pack2bf(x[1].a[2], x[1].a[3])});
+      st<NT>(reinterpret_cast<vu4*>(ov) + i, vu4{pack2bf(y[0].a[0], y[0].a[1]), pack2bf(y[0].a[2], y[0].a[3]),
+                                                 pack2bf(y[1].a[0], y[1].a[1]), pack2bf(y[1].a[2], y[1].a[3])});
     } else {
-      st4(reinterpret_cast<float*>(om) + 4 * i, x);
-      st4(reinterpret_cast<float*>(ov) + 4 * i, y);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        st4<NT>(reinterpret_cast<float*>(om) + 8 * i + 4 * k, x[k]);
+        st4<NT>(reinterpret_cast<float*>(ov) + 8 * i + 4 * k, y[k]);
+      }
     }
   }
 }
 
 }  // namespace
 
-hipError_t adamw(const AdamwArgs& a, int bits, int g_bf16, hipStream_t st) {
-  if ((bits != 8 && bits != 32) || !a.step || a.nchunks < 0 || (a.nchunks && !(a.chunks && a.m && a.v)) ||
-      (bits == 8 && a.nchunks && !a.scales) ||
-      (a.partials && (!a.norm || a.npartials < 1 || a.npartials > OPT_MAX_GRID)))
-    return hipErrorInvalidValue;
+namespace {
+// us, cold (three sets of tensors in turn), one MI355X:
+//   cached / past the caches (NT), 4096 pieces: fp32 gradients, 32-bit states: 7M weights 35.8 / 33.1, 18M
+//   100.7 / 80.6, 120M 655 / 611; 8-bit states: 7M 22.2 / 22.9, 18M 62.2 / 50.8, 120M 385 / 355.  So NT is
+//   for weights and states that do not stay in the 256 MB of the last cache anyway (OPT_NT_BYTES).  Gradients
+//   have just been written and are read through it (18M: 80.6 / 89.8 with them past it), but fp32 ones
+//   of the largest tables (120M: 611 / 607).
+//   1024 workgroups that take pieces in turn / a workgroup for each piece (FULL): 18M 80.8 / 78.2, 35M 169 / 161,
+//   70M 345 / 324, 120M 596 / 561; 8 bits: 35M 103 / 98, 120M 367 / 324.  FULL costs a launch (the step
+//   counter has one word for each of 1024 workgroups): from 8 pieces each on.
+template <int BITS, bool GB>
+void launch_adamw(const AdamwArgs& a, hipStream_t st) {
   const dim3 grid = ggrid(opt_grid(a.nchunks));
-  if (bits == 8) {
-    if (g_bf16) hipLaunchKernelGGL((adamw_kernel<8, true>), grid, dim3(TPB), 0, st, a, garg());
-    else hipLaunchKernelGGL((adamw_kernel<8, false>), grid, dim3(TPB), 0, st, a, garg());
+  constexpr int R = OPT_CHUNK / (TPB * 4), RB = OPT_CHUNK_BIG / (TPB * 4);
+  if (a.chunk == OPT_CHUNK) {
+    hipLaunchKernelGGL((adamw_kernel<BITS, GB, R, false, false>), grid, dim3(TPB), 0, st, a, garg());
+  } else if ((long long)a.nchunks * a.chunk * (BITS == 8 ? 12 : 24) < OPT_NT_BYTES) {
+    hipLaunchKernelGGL((adamw_kernel<BITS, GB, RB, false, false>), grid, dim3(TPB), 0, st, a, garg());
+  } else if (a.nchunks < 8 * OPT_MAX_GRID) {
+    hipLaunchKernelGGL((adamw_kernel<BITS, GB, RB, true, false>), grid, dim3(TPB), 0, st, a, garg());
   } else {
-    if (g_bf16) hipLaunchKernelGGL((adamw_kernel<32, true>), grid, dim3(TPB), 0, st, a, garg());
-    else hipLaunchKernelGGL((adamw_kernel<32, false>), grid, dim3(TPB), 0, st, a, garg());
+    hipLaunchKernelGGL(adamw_begin_kernel, ggrid(1), dim3(TPB), 0, st, a, garg());
+    hipLaunchKernelGGL((adamw_kernel<BITS, GB, RB, true, true>), ggrid(a.nchunks), dim3(TPB), 0, st, a, garg());
+  }
+}
+}  // namespace
+
+hipError_t adamw(const AdamwArgs& a, int bits, int g_bf16, hipStream_t st) {
+  if ((bits != 8 && bits != 32) || (a.chunk != OPT_CHUNK && a.chunk != OPT_CHUNK_BIG) || !a.step || a.nchunks < 0 ||
+      !a.norm || (a.nchunks && !(a.chunks && a.m && a.v)) || (bits == 8 && a.nchunks && !a.scales))
+    return hipErrorInvalidValue;
+  if (a.clip > 0.f && (a.partials ? a.npartials < 1 || a.npartials > OPT_MAX_GRID : a.nchunks > OPT_NORM_ONE))
+    return hipErrorInvalidValue;
+  if (bits == 8) {
+    if (g_bf16) launch_adamw<8, true>(a, st);
+    else launch_adamw<8, false>(a, st);
+  } else {
+    if (g_bf16) launch_adamw<32, true>(a, st);
+    else launch_adamw<32, false>(a, st);
   }
   return hipGetLastError();
 }
@@ -416,7 +555,7 @@ hipError_t grad_norm_partials(const OptChunk* chunks, int nchunks, int g_bf16, d
 }
 
 hipError_t grad_norm(const OptChunk* chunks, int nchunks, int g_bf16, double* partials, float* out, hipStream_t st) {
-  if (nchunks < 0 || (nchunks && !chunks) || !partials || !out) return hipErrorInvalidValue;
+  if (nchunks < 0 || (nchunks && !chunks) || (nchunks > OPT_NORM_ONE && !partials) || !out) return hipErrorInvalidValue;
   if (nchunks <= OPT_NORM_ONE) {
     if (g_bf16) hipLaunchKernelGGL((grad_norm_kernel<true, true>), dim3(1), dim3(TPB), 0, st, chunks, nchunks,
                                    partials, out, GroupArg{0, 1, 0});
@@ -440,10 +579,16 @@ hipError_t adamw_decode(const unsigned char* m, const unsigned char* v, const un
   if (n < 0 || n % OPT_BLOCK) return hipErrorInvalidValue;
   if (n == 0) return hipSuccess;
   if (!m || !v || !scales || !om || !ov) return hipErrorInvalidValue;
-  const long long n4 = n / 4, blocks = (n4 + TPB - 1) / TPB;
-  const dim3 grid((unsigned)(blocks < 8192 ? blocks : 8192));
-  if (out_bf16) hipLaunchKernelGGL(adamw_decode_kernel<true>, grid, dim3(TPB), 0, st, m, v, scales, n4, om, ov);
-  else hipLaunchKernelGGL(adamw_decode_kernel<false>, grid, dim3(TPB), 0, st, m, v, scales, n4, om, ov);
+  const long long n8 = n / 8, blocks = (n8 + TPB - 1) / TPB;
+  const dim3 grid((unsigned)blocks);
+  const bool nt = n * (out_bf16 ? 6 : 10) >= OPT_NT_BYTES;
+  if (out_bf16) {
+    if (nt) hipLaunchKernelGGL((adamw_decode_kernel<true, true>), grid, dim3(TPB), 0, st, m, v, scales, n8, om, ov);
+    else hipLaunchKernelGGL((adamw_decode_kernel<true, false>), grid, dim3(TPB), 0, st, m, v, scales, n8, om, ov);
+  } else {
+    if (nt) hipLaunchKernelGGL((adamw_decode_kernel<false, true>), grid, dim3(TPB), 0, st, m, v, scales, n8, om, ov);
+    else hipLaunchKernelGGL((adamw_decode_kernel<false, false>), grid, dim3(TPB), 0, st, m, v, scales, n8, om, ov);
+  }
   return hipGetLastError();
 }
 

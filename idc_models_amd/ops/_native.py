@@ -213,10 +213,10 @@ class AdamwArgs(C.Structure):
     _fields_ = [(n, vp) for n in ("chunks", "m", "v", "scales", "step", "partials", "norm", "skip", "hostflag")] + \
                [("log_b1", C.c_double), ("log_b2", C.c_double)] + \
                [(n, cf) for n in ("b1", "omb1", "b2", "omb2", "lr", "eps", "lr_wd", "grad_scale", "clip")] + \
-               [("nchunks", ci), ("npartials", ci)]
+               [("nchunks", ci), ("npartials", ci), ("chunk", ci), ("pad", ci)]
 
 
-OPT_CHUNK, OPT_MAX_GRID, OPT_BLOCK = 2048, 1024, 64  # csrc/kernels/adamw.h
+OPT_CHUNK, OPT_CHUNK_BIG, OPT_MAX_GRID, OPT_BLOCK, OPT_NORM_ONE = 2048, 4096, 1024, 64, 8  # csrc/kernels/adamw.h
 OPT_DECAY, OPT_VEC = 1, 2
 
 
@@ -263,7 +263,8 @@ def _verify(ext):
             or ext.OP_DENSE_INFER != OP_DENSE_INFER:
         raise RuntimeError("native op-kind table drifted (OP_DENSE_STAGE / OP_MB_CHAIN)")
     if (ext.OP_ADAMW, ext.OP_GRAD_NORM) != (OP_ADAMW, OP_GRAD_NORM) \
-            or (ext.OPT_CHUNK, ext.OPT_MAX_GRID, ext.OPT_BLOCK) != (OPT_CHUNK, OPT_MAX_GRID, OPT_BLOCK):
+            or (ext.OPT_CHUNK, ext.OPT_CHUNK_BIG, ext.OPT_MAX_GRID, ext.OPT_BLOCK, ext.OPT_NORM_ONE) \
+            != (OPT_CHUNK, OPT_CHUNK_BIG, OPT_MAX_GRID, OPT_BLOCK, OPT_NORM_ONE):
         raise RuntimeError("native multi-tensor optimizer constants drifted")
     sizes = ext.struct_sizes()
     for name, cls in _STRUCTS.items():

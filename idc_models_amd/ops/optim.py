@@ -54,24 +54,29 @@ def _span(t: torch.Tensor) -> Tuple[int, int]:
     return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
 
 
+def chunk_size(sizes: Sequence[int]) -> int:
+    """Elements of a full piece of a table (csrc/kernels/adamw.h)."""
+    return nat.OPT_CHUNK_BIG if sum(sizes) >= nat.OPT_MAX_GRID * nat.OPT_CHUNK_BIG else nat.OPT_CHUNK
+
+
 def chunk_table(sizes: Sequence[int], w_ptrs: Sequence[int], g_ptrs: Sequence[int], grad_bytes: int,
-                decay: Sequence[bool]) -> Tuple[np.ndarray, np.ndarray, int]:
-    """``(pieces, offsets, numel)``: the OptChunk records of tensors with these sizes and addresses,
-    every tensor's place in the flat state (multiples of 64), and the state's length."""
+                decay: Sequence[bool], chunk: int) -> Tuple[np.ndarray, np.ndarray, int]:
+    """``(pieces, offsets, numel)``: the OptChunk records (of at most ``chunk`` elements) of tensors with
+    these sizes and addresses, every tensor's place in the flat state (multiples of 64), and the state's length."""
     n = np.asarray(sizes, dtype=np.int64)
     room = (n + nat.OPT_BLOCK - 1) // nat.OPT_BLOCK * nat.OPT_BLOCK
     offsets = np.concatenate([[0], np.cumsum(room)])
     w, g = np.asarray(w_ptrs, dtype=np.uint64), np.asarray(g_ptrs, dtype=np.uint64)
     vec = (w % 16 == 0) & (g % (4 * grad_bytes) == 0)
     flags = np.asarray(decay, dtype=bool) * nat.OPT_DECAY + vec * nat.OPT_VEC
-    count = (n + nat.OPT_CHUNK - 1) // nat.OPT_CHUNK
+    count = (n + chunk - 1) // chunk
     of = np.repeat(np.arange(len(n)), count)  # the tensor of every piece
-    start = (np.arange(len(of)) - np.repeat(np.cumsum(count) - count, count)) * nat.OPT_CHUNK
+    start = (np.arange(len(of)) - np.repeat(np.cumsum(count) - count, count)) * chunk
     out = np.zeros(len(of), dtype=_CHUNK)
     out["w"] = np.where(w[of] != 0, w[of] + (start * 4).astype(np.uint64), 0)
     out["g"] = g[of] + (start * grad_bytes).astype(np.uint64)
     out["base"] = offsets[:-1][of] + start
-    out["n"] = np.minimum(n[of] - start, nat.OPT_CHUNK)
+    out["n"] = np.minimum(n[of] - start, chunk)
     out["flags"] = flags[of]
     return out, offsets[:-1], int(offsets[-1])
 
@@ -128,9 +133,10 @@ class TensorTable:
             raise ValueError("TensorTable needs tensors on a GPU")
         self.grads, self.params = grads, params
         sizes = [g.numel() for g in grads]
+        self.chunk = chunk_size(sizes)
         pieces, offsets, self.numel = chunk_table(
             sizes, [p.data_ptr() for p in params] if params is not None else [0] * len(grads),
-            [g.data_ptr() for g in grads], self.grad_dtype.itemsize, decay)
+            [g.data_ptr() for g in grads], self.grad_dtype.itemsize, decay, self.chunk)
         if len(pieces) >= 1 << 31:
             raise ValueError("too many elements for one table")
         self.sizes, self.offsets = sizes, offsets.tolist()
@@ -167,11 +173,12 @@ class AdamWState:
         self.scales = torch.zeros(room // nat.OPT_BLOCK, 2, dtype=torch.uint8,
                                   device=self.device)[:self.numel // nat.OPT_BLOCK] if bits == 8 else None
         self.step = torch.zeros(nat.OPT_MAX_GRID, dtype=torch.int32, device=self.device)
-        self.norm = torch.zeros((), dtype=torch.float32, device=self.device)
+        self._work = torch.zeros(4, dtype=torch.float32, device=self.device)
+        self.norm = self._work[0]
         self.partials = torch.zeros(nat.OPT_MAX_GRID, dtype=torch.float64, device=self.device)
         a = self._args = nat.AdamwArgs()
         a.m, a.v, a.scales = self.m.data_ptr(), self.v.data_ptr(), nat.ptr(self.scales)
-        a.step, a.norm = self.step.data_ptr(), self.norm.data_ptr()
+        a.step, a.norm = self.step.data_ptr(), self._work.data_ptr()
 
     def tensors(self) -> dict:
         """What a checkpoint keeps."""
@@ -239,7 +246,8 @@ def _on(device: torch.device):
 
 
 def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    # current_stream(device).cuda_stream builds a Stream object for its handle: 1.7 of a 6.7 us call
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def check_adamw(lr: float, beta_1: float, beta_2: float, epsilon: float, weight_decay: float, clip_norm: float) -> None:
@@ -255,14 +263,14 @@ def check_adamw(lr: float, beta_1: float, beta_2: float, epsilon: float, weight_
 def set_adamw_args(a: "nat.AdamwArgs", table: TensorTable, state: AdamWState, lr: float, beta_1: float, beta_2: float,
                    epsilon: float, weight_decay: float, grad_scale: float, clip_norm: float, skip: int = 0,
                    hostflag: int = 0) -> "nat.AdamwArgs":
-    a.chunks, a.nchunks = table.chunks.data_ptr(), table.nchunks
+    a.chunks, a.nchunks, a.chunk = table.chunks.data_ptr(), table.nchunks, table.chunk
     a.b1, a.b2, a.omb1, a.omb2 = beta_1, beta_2, 1.0 - beta_1, 1.0 - beta_2
     a.log_b1 = math.log(beta_1) if beta_1 else -math.inf
     a.log_b2 = math.log(beta_2) if beta_2 else -math.inf
     a.lr, a.eps, a.lr_wd = lr, epsilon, lr * weight_decay
     a.grad_scale, a.clip = grad_scale, clip_norm
-    if clip_norm:
-        a.partials, a.npartials = state.partials.data_ptr(), min(max(table.nchunks, 1), nat.OPT_MAX_GRID)
+    if clip_norm and table.nchunks > nat.OPT_NORM_ONE:  # grad_norm's partial sums; else the step sums by itself
+        a.partials, a.npartials = state.partials.data_ptr(), min(table.nchunks, nat.OPT_MAX_GRID)
     else:
         a.partials, a.npartials = 0, 0
     a.skip, a.hostflag = skip, hostflag
@@ -277,8 +285,8 @@ def adamw_(table: TensorTable, state: AdamWState, lr: float, beta_1: float = 0.9
         t += 1;  g = grad_scale * grad;  m = beta_1*m + (1-beta_1)*g;  v = beta_2*v + (1-beta_2)*g^2
         w -= lr*weight_decay*w + lr*sqrt(1-beta_2^t)/(1-beta_1^t) * m/(sqrt(v)+epsilon)
 
-    ``clip_norm`` > 0 scales g down to that global norm (one launch more, nothing is read back; a norm
-    that is not finite makes every gradient NaN).  ``skip``: an int32 tensor on the device; if its
+    ``clip_norm`` > 0 scales g down to that global norm (one launch more for all but small tables, nothing
+    is read back; a norm that is not finite makes every gradient NaN).  ``skip``: an int32 tensor on the device; if its
     first word is not zero the call changes nothing."""
     check_adamw(lr, beta_1, beta_2, epsilon, weight_decay, clip_norm)
     if table.params is None:
@@ -292,7 +300,7 @@ def adamw_(table: TensorTable, state: AdamWState, lr: float, beta_1: float = 0.9
     ext = nat.require()
     with _on(table.device):
         stream = _stream(table.device)
-        if clip_norm:
+        if a.partials:
             ext.grad_norm(a.chunks, table.nchunks, table._bf16, a.partials, 0, stream)
         ext.adamw(ctypes.addressof(a), state.bits, table._bf16, stream)
 
@@ -301,10 +309,11 @@ def global_norm(table: TensorTable) -> torch.Tensor:
     """sqrt of the sum of the squares of all the table's gradients: an fp32 tensor without axes.
     Sums in fp64 in a fixed order (the same bits every time)."""
     dev = table.device
-    partials = torch.empty(nat.OPT_MAX_GRID, dtype=torch.float64, device=dev)
+    many = table.nchunks > nat.OPT_NORM_ONE
+    partials = torch.empty(nat.OPT_MAX_GRID, dtype=torch.float64, device=dev) if many else None
     out = torch.empty((), dtype=torch.float32, device=dev)
     ext = nat.require()
     with _on(dev):
-        ext.grad_norm(table.chunks.data_ptr(), table.nchunks, table._bf16, partials.data_ptr(), out.data_ptr(),
+        ext.grad_norm(table.chunks.data_ptr(), table.nchunks, table._bf16, nat.ptr(partials), out.data_ptr(),
                       _stream(dev))
     return out

@@ -60,10 +60,10 @@ def test_refused_hyperparameters():
 
 def test_pieces_cover_every_element_once():
     sizes = [0, 1, 64, 65, 2047, 2048, 2049, 10 * 2048 + 1, 0]
-    for grad_bytes in (4, 2):
+    for grad_bytes, chunk in ((4, 2048), (2, 2048), (4, 4096)):
         w = np.cumsum([4096] + [4 * n + 4096 for n in sizes[:-1]]) // 16 * 16 + 4 * np.arange(len(sizes)) % 3
         g = np.cumsum([1 << 20] + [grad_bytes * n + 64 for n in sizes[:-1]]) // 16 * 16
-        pieces, offsets, numel = optim.chunk_table(sizes, w, g, grad_bytes, [i % 2 == 0 for i in range(len(sizes))])
+        pieces, offsets, numel = optim.chunk_table(sizes, w, g, grad_bytes, [i % 2 == 0 for i in range(len(sizes))], chunk)
         assert offsets.tolist() == np.concatenate([[0], np.cumsum([orc.pad64(n) for n in sizes])[:-1]]).tolist()
         assert numel == sum(orc.pad64(n) for n in sizes)
         k = 0
@@ -72,7 +72,7 @@ def test_pieces_cover_every_element_once():
             while at < n:
                 c = pieces[k]
                 assert c["w"] == w[i] + 4 * at and c["g"] == g[i] + grad_bytes * at and c["base"] == offsets[i] + at
-                assert c["n"] == min(2048, n - at) and c["base"] % 64 == 0
+                assert c["n"] == min(chunk, n - at) and c["base"] % 64 == 0
                 assert bool(c["flags"] & 1) == (i % 2 == 0)
                 assert bool(c["flags"] & 2) == (w[i] % 16 == 0 and g[i] % (4 * grad_bytes) == 0)
                 assert c["base"] + orc.pad64(int(c["n"])) <= numel

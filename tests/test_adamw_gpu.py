@@ -161,12 +161,65 @@ def test_step_matches_the_formula(bits, grad_dtype, layout):
 
 
 def test_more_pieces_than_workgroups():
-    sizes = [2048 * 700 + 3, 2048 * 900, 77]
-    for bits in (32, 8):
+    """More pieces than workgroups; the larger pieces of large tables; beyond the caches."""
+    for sizes, bits in (([2048 * 700 + 3, 2048 * 900, 77], 32), ([2048 * 700 + 3, 2048 * 900, 77], 8),
+                        ([4096 * 700 + 3, 4096 * 400, 77], 32), ([4096 * 700 + 3, 4096 * 400, 77], 8),
+                        ([4096 * 2800 + 3, 77], 8)):
         params, grads, _ = make(sizes, "own", seed=9)
-        table, st = start(params, grads, bits, 5, [True, False, True])
-        assert table.nchunks > 1024
-        check_step(params, grads, table, st, [True, False, True], 1.0, 1.0)
+        decay = [i != 1 for i in range(len(sizes))]
+        table, st = start(params, grads, bits, 5, decay)
+        assert table.nchunks > 1024 and table.chunk == (2048 if sizes[0] < 4096 * 700 else 4096)
+        check_step(params, grads, table, st, decay, 1.0, 1.0)
+
+
+@pytest.mark.parametrize("grad_dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_the_largest_tables(bits, grad_dtype):
+    """A workgroup for each piece, and a launch that counts: two clipped steps; the ends of both
+    tensors against the oracle."""
+    from idc_models_amd.ops import optim
+    n = [8192 * 4096 + 4096 + 5, 777]
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    params = [torch.randn(k, device=DEV, generator=gen) for k in n]
+    grads = [torch.randn(k, device=DEV, generator=gen).to(grad_dtype) for k in n]
+    table = optim.TensorTable(grads, params, decay=[True, False])
+    st = optim.AdamWState(table, bits=bits)
+    assert table.nchunks >= 8192
+    word = torch.ones(1, dtype=torch.int32, device=DEV)
+    before = params[1].clone()
+    optim.adamw_(table, st, **HYPER, skip=word, clip_norm=10.0)
+    assert int(st.step[0]) == 0 and torch.equal(before, params[1]) and int(st.m.view(torch.uint8).max()) == 0
+    total = math.sqrt(sum(float(g.double().square().sum()) for g in grads))
+    first = (n[0] - 10000) // 64 * 64
+    parts = [(0, 0, 0, 8192), (0, first, first, n[0]), (1, 0, table.offsets[1], 777)]  # tensor, from, place, to
+    for t in (1, 2):
+        olds = [(params[i][a:b].double().cpu(), grads[i][a:b].double().cpu()) for i, a, _, b in parts]
+        states = [slice_values(st, at, orc.pad64(b - a)) for _, a, at, b in parts]
+        optim.adamw_(table, st, **HYPER, clip_norm=10.0)
+        assert float(st.norm) == pytest.approx(total, rel=2 * orc.U) and bool((st.step == t).all())
+        for (i, a, at, b), (w0, g), (m0, r0) in zip(parts, olds, states):
+            k, pad = b - a, orc.pad64(b - a)
+            ext = lambda x: torch.cat([x, torch.zeros(pad - k, dtype=torch.float64)])
+            w1, m1, v1, root, tw, tm, tv, tr = orc.step(ext(w0), ext(g), m0, r0 * r0, t, HYPER["lr"], 0.9, 0.999, 1e-7, 0.1,
+                                                        torch.full((pad,), float(i == 0), dtype=torch.float64), 1.0, 10.0, total)
+            orc.within(params[i][a:b], w1[:k], tw[:k])
+            m, r = slice_values(st, at, pad)
+            if bits == 32:
+                orc.within(m, m1, tm)
+                orc.within(r, root, tr + orc.U * root)
+                continue
+            low, high = orc.hash_bits(pad, t, start=at)
+            slack = torch.where(m1 == 0, torch.zeros_like(m1), tm / m1.abs().clamp(min=1e-300)).clamp(min=32 * orc.U, max=0.5)
+            for have, (lo, hi, open_) in ((m, bounds_each(m1, 3, low, slack)), (r, orc.code_bounds(root, 4, high, 16 * orc.U))):
+                assert bool(((have == lo) | (have == hi) | open_).all())
+
+
+def slice_values(st, at, n):
+    """First moments and roots (fp64) of n places of the state from a multiple of 64 on."""
+    if st.bits == 32:
+        return st.m[at:at + n].double().cpu(), st.v[at:at + n].double().sqrt().cpu()
+    sc = st.scales[at // 64:(at + n) // 64].cpu()
+    return (orc.code_values(st.m[at:at + n].cpu(), sc[:, 0], 3), orc.code_values(st.v[at:at + n].cpu(), sc[:, 1], 4))
 
 
 @pytest.mark.parametrize("bits", [32, 8])
