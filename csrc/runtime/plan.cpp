@@ -96,7 +96,8 @@ enum OpKind : int {
   OP_MB_INFER = 31,
   // a whole DenseNet dense block in inference mode (dense_infer.hip): payload DenseInferArgs
   OP_DENSE_INFER = 32,
-  // multi-tensor AdamW step (adamw.hip): payload AdamwArgs, i[0] state bits, i[1] bf16 gradients
+  // multi-tensor AdamW step (adamw.hip): payload AdamwArgs, i[0] state bits, i[1] bf16 gradients, f[0]
+  // learning rate, f[1] weight decay; p[0] and i[2]: the piece table and its length again
   OP_ADAMW = 33,
   // partial sums of the squared gradients (adamw.hip): p[0] device OptChunk[i[0]], p[1] partials,
   // i[1] bf16 gradients
@@ -642,7 +643,13 @@ class Plan {
                       reinterpret_cast<const int*>(op.p[3]), reinterpret_cast<int*>(op.p[4]), st),
               "rmsprop");
         break;
-      case OP_ADAMW: check(adamw(as<AdamwArgs>(op), op.i[0], op.i[1], st), "adamw"); break;
+      case OP_ADAMW: {
+        AdamwArgs a = as<AdamwArgs>(op);
+        a.lr = op.f[0];  // (set_float changes it)
+        a.lr_wd = op.f[0] * op.f[1];
+        check(adamw(a, op.i[0], op.i[1], st), "adamw");
+        break;
+      }
       case OP_GRAD_NORM:
         check(grad_norm_partials(reinterpret_cast<const OptChunk*>(op.p[0]), op.i[0], op.i[1],
                                  reinterpret_cast<double*>(op.p[1]), st),

@@ -146,10 +146,7 @@ def load_checkpoint(model, path: str) -> dict:
     opt = state.get("optimizer")
     if opt and model.optimizer is not None and opt["name"] == model.optimizer.name:
         model.optimizer.iterations = opt["iterations"]
-        for k, v in opt["slots"].items():
-            cur = model.optimizer.state_tensors().get(k)
-            if cur is not None and cur.shape == v.shape:
-                cur.copy_(v.to(cur.device))
+        model.optimizer.load_slots(opt["slots"])
     if "rng_cpu" in state:
         torch.set_rng_state(state["rng_cpu"])
     return {"epoch": state.get("epoch", 0), **state.get("extra", {})}

@@ -37,6 +37,7 @@ def main(argv=None):
     d.add_argument("--epochs", type=int, default=None, help="initial (= fine-tune) epochs")
     d.add_argument("--steps-per-epoch", type=int, default=None)
     d.add_argument("--arch", default=None)
+    d.add_argument("--optimizer", default=None, choices=[None, "rmsprop", "adamw"])
     f = sub.add_parser("fed", help="federated averaging (fed_model.py)")
     f.add_argument("path")
     f.add_argument("rounds", type=int)
@@ -74,6 +75,8 @@ def main(argv=None):
             kw["steps_per_epoch"] = a.steps_per_epoch
         if a.arch:
             kw["arch"] = a.arch
+        if a.optimizer:
+            kw["optimizer"] = a.optimizer
         if "input_shape" in kw:
             kw["input_shape"] = tuple(kw["input_shape"])
         run_transfer_learning(TransferConfig(**kw))

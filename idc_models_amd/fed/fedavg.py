@@ -7,7 +7,8 @@ TFF 0.12 semantics reproduced:
 * the server broadcasts its model; each client starts from it with a FRESH client optimizer,
   trains one local epoch over its dataset, and reports the delta of its TRAINABLE weights with
   weight = number of examples (a client whose delta is non-finite gets weight 0);
-* the server applies the example-weighted mean delta with SGD(lr=1.0) (``server_optimizer_fn``);
+* the server applies the example-weighted mean delta with SGD(lr=1.0) (``server_optimizer_fn``; an
+  ``AdamW`` takes minus the mean delta as its gradient, its moments live in ``ServerState.optimizer_state``);
 * non-trainable weights (BN moving statistics) are not aggregated, unless
   ``average_bn_stats=True`` (documented deviation for BN backbones, SURVEY Q16);
 * metrics are example-weighted sums across clients, reported as OrderedDict(binary_accuracy, loss).
@@ -138,9 +139,13 @@ class FedAvgProcess:
         self._more_workers = []
         self.client_optimizer_fn = client_optimizer_fn
         self.server_lr = 1.0
+        self._server_opt = self._server_arena = None
         if server_optimizer_fn is not None:
             opt = server_optimizer_fn()
             self.server_lr = float(getattr(opt, "learning_rate", 1.0))
+            from ..engine.optimizers import AdamW
+            if isinstance(opt, AdamW):
+                self._server_opt = opt
         self.average_bn_stats = average_bn_stats
         self.local_epochs = local_epochs
         self.loss = loss
@@ -306,6 +311,30 @@ class FedAvgProcess:
     def _load(self, m, weights: ModelWeights):
         _load_into(m, weights)
 
+    @torch.no_grad()
+    def _adaptive_server_step(self, state: ServerState, mean_delta: torch.Tensor):
+        """One AdamW step of the server's weights with minus the mean delta as the gradient (every
+        rank takes the same step from the same sums).  Returns (flat new weights, optimizer state)."""
+        from ..engine.arena import ParamArena
+        opt, arena = self._server_opt, self._server_arena
+        sizes = [w.numel() for w in state.model.trainable]
+        if arena is None or [p.shape for p in arena.params] != [w.shape for w in state.model.trainable]:
+            arena = ParamArena([torch.nn.Parameter(w.detach().to(mean_delta.device).clone())
+                                for w in state.model.trainable])
+            opt.bind(arena)
+            self._server_arena = arena
+        # multi-tensor copies, as in _load_into
+        torch._foreach_copy_(arena.params, [w.to(mean_delta.device) for w in state.model.trainable])
+        torch._foreach_copy_([p.grad for p in arena.params],
+                             [d.view(p.shape) for p, d in zip(arena.params, mean_delta.split(sizes))])
+        arena.grad.neg_()
+        opt.reset_state()
+        if state.optimizer_state:
+            opt.load_slots(state.optimizer_state)
+        opt.step(arena)
+        return (torch.cat([p.detach().reshape(-1) for p in arena.params]),
+                {k: t.clone() for k, t in opt.state_tensors().items()})
+
     # -------------------------------------------------------------- round
     def next(self, state: ServerState, federated_train_data: Sequence, participating=None):
         """One round.  ``participating``: indices of the clients that report this round (default
@@ -376,9 +405,13 @@ class FedAvgProcess:
         if world > 1:
             comm.all_reduce_packed_(clear)
         total = float(n_sum.item())
+        opt_state = state.optimizer_state
         if total > 0:
             mean_delta = delta_sum / total
-            new_flat = flat_server + self.server_lr * mean_delta
+            if self._server_opt is not None:
+                new_flat, opt_state = self._adaptive_server_step(state, mean_delta)
+            else:
+                new_flat = flat_server + self.server_lr * mean_delta
         else:
             new_flat = flat_server
         # the new server weights are VIEWS of one fresh flat buffer each (trainable / statistics):
@@ -398,7 +431,7 @@ class FedAvgProcess:
         for i, name in enumerate(self.metric_names):
             metrics[name] = float(met[1 + i].item() / total) if total else 0.0
         metrics["loss"] = float(met[0].item() / total) if total else 0.0
-        return ServerState(ModelWeights(new_tr, new_ntr), state.round_num + 1, state.optimizer_state), metrics
+        return ServerState(ModelWeights(new_tr, new_ntr), state.round_num + 1, opt_state), metrics
 
 
 def build_federated_averaging_process(model_fn, client_optimizer_fn, server_optimizer_fn=None, **kw):

@@ -20,7 +20,7 @@ import torch
 
 from ..data import (ArrayDataset, cifar10_dataset, idc_dataset, prepare_for_training, split,
                     synthetic_dataset)
-from ..engine import Model, RMSprop
+from ..engine import AdamW, Model, RMSprop
 from ..models import build_model
 from ..utils.plot import log as plot_log
 from ..utils.timer import Timer
@@ -49,6 +49,18 @@ class TransferConfig:
     ylim: Optional[tuple] = None
     steps_per_epoch: Optional[int] = None
     verbose: int = 0
+    optimizer: str = "rmsprop"         # rmsprop (the reference's) | adamw
+    optimizer_args: Optional[dict] = None  # further arguments, e.g. weight_decay, global_clipnorm, state_bits
+
+
+OPTIMIZERS = {"rmsprop": RMSprop, "adamw": AdamW}
+
+
+def make_optimizer(name: str, learning_rate: float, args: Optional[dict] = None):
+    """A recipe's optimizer by its name (fresh state)."""
+    if name not in OPTIMIZERS:
+        raise ValueError(f"unknown optimizer {name!r}: one of {', '.join(sorted(OPTIMIZERS))}")
+    return OPTIMIZERS[name](learning_rate, **(args or {}))
 
 
 PRESETS = {
@@ -112,7 +124,7 @@ def run_transfer_learning(cfg: TransferConfig, printer=print):
         net = build_model(cfg.arch, cfg.input_shape, cfg.num_classes, seed=cfg.seed)
         net.base.trainable = False
         model = Model(net, strategy)
-        model.compile(RMSprop(cfg.base_learning_rate), loss, ["accuracy"],
+        model.compile(make_optimizer(cfg.optimizer, cfg.base_learning_rate, cfg.optimizer_args), loss, ["accuracy"],
                       keras_compat_accuracy=cfg.keras_compat_accuracy, backend=cfg.backend)
     loss0, acc0 = model.evaluate(val, steps=cfg.validation_steps)
     if strategy.is_chief:
@@ -127,7 +139,7 @@ def run_transfer_learning(cfg: TransferConfig, printer=print):
     with strategy.scope():
         for layer in net.base.layers[:cfg.fine_tune_at]:
             layer.trainable = False
-        model.compile(RMSprop(cfg.base_learning_rate / 10), loss, ["accuracy"],
+        model.compile(make_optimizer(cfg.optimizer, cfg.base_learning_rate / 10, cfg.optimizer_args), loss, ["accuracy"],
                       keras_compat_accuracy=cfg.keras_compat_accuracy, backend=cfg.backend)
     total = cfg.initial_epochs + cfg.fine_tune_epochs
     with Timer(f"Fine-tuning with {n} devices", printer if strategy.is_chief else None):

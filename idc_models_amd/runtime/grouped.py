@@ -15,7 +15,7 @@ every launch covers all K clients:
 * copy g of any buffer is then ``copy 0 + g * stride``: the kernels take a ``GroupArg`` and shift
   every pointer they dereference by ``(blockIdx.z / zn) * stride`` (``csrc/kernels/common.h``), and
   the launchers multiply their grid's z extent by K (``Plan.set_groups``);
-* per-client state (weights, BN statistics, RMSprop slots, inputs, labels, losses) is addressed
+* per-client state (weights, BN statistics, optimizer slots, inputs, labels, losses) is addressed
   from Python as ``[K, ...]`` strided views of the slab (``view``).
 
 Reference: TFF runs the clients of a round one after another in one process
@@ -38,12 +38,13 @@ _PAYLOAD = {
     nat.OP_POOL_BWD: nat.PoolBwdArgs, nat.OP_HEAD_FWD: nat.HeadArgs, nat.OP_HEAD_BWD: nat.HeadBwdArgs,
     nat.OP_BN_APPLY: nat.BnArgs, nat.OP_DW_FWD: nat.DwArgs, nat.OP_DW_BWD_DATA: nat.DwArgs,
     nat.OP_DW_WGRAD: nat.DwArgs, nat.OP_MLP_FWD: nat.Mlp2Args, nat.OP_MLP_BWD: nat.Mlp2Args,
-    nat.OP_DENSE_STAGE: nat.DenseStageArgs, nat.OP_MB_CHAIN: nat.MbChainArgs,
+    nat.OP_DENSE_STAGE: nat.DenseStageArgs, nat.OP_MB_CHAIN: nat.MbChainArgs, nat.OP_ADAMW: nat.AdamwArgs,
 }
 # descriptor-table ops: (ptr slot of the table, int slot of its length, entry type)
 _TABLES = {nat.OP_BN_MOVING: (0, 0, nat.BnMovingDesc), nat.OP_STATS_SHIFT: (0, 0, nat.ShiftDesc),
            nat.OP_CAST: (0, 0, nat.CastEntry), nat.OP_WGRAD_BATCH: (0, 0, nat.WgBatchEntry),
-           nat.OP_DENSE_STAGE: (0, 1, nat.DenseLayerDesc), nat.OP_MB_CHAIN: (0, 2, nat.MbPhaseDesc)}
+           nat.OP_DENSE_STAGE: (0, 1, nat.DenseLayerDesc), nat.OP_MB_CHAIN: (0, 2, nat.MbPhaseDesc),
+           nat.OP_ADAMW: (0, 2, nat.OptChunk), nat.OP_GRAD_NORM: (0, 0, nat.OptChunk)}
 
 
 def _struct_ptrs(obj, path=""):

@@ -3,7 +3,7 @@
 ``FusedProgram`` = one static plan for (model, batch, training, input dtype):
   segment ``fwd``  input staging -> convs/pools (fused BN/act) -> head loss -> BN moving update
   segment ``bwd``  grad-arena memset -> head bwd -> dgrad/wgrad/BN-bwd in reverse order
-  segment ``opt``  fused RMSprop over the flat arena -> bf16 weight re-cast (ONE launch each)
+  segment ``opt``  fused RMSprop or AdamW over the flat arena -> bf16 weight re-cast (ONE launch each)
 Each segment is captured into a HIP graph on first use and replayed afterwards.  Under data
 parallelism the backward segment is split at bucket boundaries so each bucket's RCCL all-reduce
 is launched while the remaining backward segments run.
@@ -16,7 +16,7 @@ from typing import Dict, List, Optional, Tuple
 import torch
 
 from ..engine.losses import BinaryCrossentropy, CategoricalCrossentropy, SparseCategoricalCrossentropy
-from ..engine.optimizers import RMSprop
+from ..engine.optimizers import AdamW
 from ..ops import _native as nat
 from ..utils import trace
 from .builder import Builder
@@ -62,14 +62,14 @@ def fused_supported(net, loss) -> bool:
 def persistent_allowed(model, training: bool) -> bool:
     """Whether a program may build persistent (work-queue) launches.  A persistent launch that
     gives up leaves stale stage outputs and relies on the step's update being skipped through the
-    step guard word: only the fused RMSprop reads that word (a host optimizer would apply the stale
-    update), and only the native communicator's guard all-reduce makes every replica skip
+    step guard word: only the fused optimizers (RMSprop, AdamW) read that word (a host optimizer would apply
+    the stale update), and only the native communicator's guard all-reduce makes every replica skip
     together (the torch bucketer path and central storage would let the other replicas apply
     gradients that include the stale contribution).  Evaluation programs are unaffected."""
     if not training or not model.arena.params:
         return True
     opt = model.optimizer
-    host_opt = not isinstance(opt, RMSprop) or bool(opt.momentum) or bool(opt.centered)
+    host_opt = not opt.native_step
     st = model.strategy
     unguarded_dp = st.active and (getattr(st, "native_comm", None) is None
                                   or getattr(st, "central_storage", False))
@@ -170,7 +170,7 @@ class FusedProgram:
         self.nonfinite_status = None
         if training and model.arena.params:
             opt = model.optimizer
-            self.host_optimizer = not isinstance(opt, RMSprop) or bool(opt.momentum) or bool(opt.centered)
+            self.host_optimizer = not opt.native_step
             flag = 0
             # persistent dense-stage launches OR 2 into the step guard word when they give up
             # (csrc/kernels/persist.h note_fail): RMSprop then skips the step's update, so stale
@@ -192,7 +192,6 @@ class FusedProgram:
                 b.emit(nat.OP_FINITE_CHECK, ints=(0,), longs=(model.arena.numel,),
                        ptrs=(model.arena.grad.data_ptr(), flag))
             if not self.host_optimizer:
-                ms = opt.ms
                 hflag = 0
                 if flag and flag == guard and not b.grouped and torch.cuda.is_available():
                     # a skip caused by a give-up on any rank raises this rank's host flag too
@@ -200,10 +199,13 @@ class FusedProgram:
                         from .builder import _host_flag_slot
                         b.host_flag = _host_flag_slot()
                     hflag = b.host_flag
-                b.emit(nat.OP_RMSPROP, floats=(opt.learning_rate, opt.rho, opt.epsilon, grad_scale),
-                       longs=(model.arena.numel,),
-                       ptrs=(model.arena.data.data_ptr(), model.arena.grad.data_ptr(), ms.data_ptr(), flag,
-                             hflag))
+                if isinstance(opt, AdamW):
+                    self._emit_adamw(b, opt, grad_scale, flag, hflag)
+                else:
+                    b.emit(nat.OP_RMSPROP, floats=(opt.learning_rate, opt.rho, opt.epsilon, grad_scale),
+                           longs=(model.arena.numel,),
+                           ptrs=(model.arena.data.data_ptr(), model.arena.grad.data_ptr(), opt.ms.data_ptr(), flag,
+                                 hflag))
             if b.cast_tr_n:
                 b.emit(nat.OP_CAST, ints=(b.cast_tr_n,), longs=(b.cast_tr_total,),
                        ptrs=(b.cast_tr_dev.data_ptr(), b.cast_tr_map.data_ptr()))
@@ -232,7 +234,7 @@ class FusedProgram:
         default_flush = "0" if b.grouped and big else "2" if big else "4" if n_bwd_main >= 64 else "0"
         self.plan.set_side_flush(int(os.environ.get("IDC_SIDE_FLUSH", default_flush)))
         self.seg: Dict[str, Tuple[int, int]] = {}
-        self.rms_index = None
+        self.opt_index = None
         op_index = 0
         self.bwd_marks = []
         mark_at = {}
@@ -292,8 +294,8 @@ class FusedProgram:
                 kind, ints, ptrs = nat.OP_BN_MOVING, [len(b.moving), b.moving_maxc], [b.moving_dev.data_ptr()]
             if kind == nat.OP_MEMSET and ptrs[0] == b.stats_arena.data_ptr():
                 longs = [max(b._stats_size, 4) * 4]
-            if kind == nat.OP_RMSPROP:
-                self.rms_index = op_index
+            if kind in (nat.OP_RMSPROP, nat.OP_ADAMW):
+                self.opt_index = op_index
             self.plan.add(kind, raw, ints, floats, longs, ptrs, lane)
             op_index += 1
         if cur == "bwd":
@@ -351,6 +353,19 @@ class FusedProgram:
             autotune_plan(self.plan, self.stream, verbose=os.environ.get("IDC_TUNE_VERBOSE") == "1",
                           reset_tickets=b.reset_tickets, slab_floats=b.SLAB_FLOATS)
         b.reset_tickets()  # split-K tickets count modulo the op's split: start every op aligned
+
+    @staticmethod
+    def _emit_adamw(b, opt, grad_scale: float, skip: int, hostflag: int):
+        from ..ops import optim
+        t, st = opt.table, opt.state
+        a = optim.set_adamw_args(nat.AdamwArgs.from_buffer_copy(st._args), t, st, opt.learning_rate, opt.beta_1,
+                                 opt.beta_2, opt.epsilon, opt.weight_decay, grad_scale, opt.clip_norm, skip, hostflag)
+        bf16 = int(t.grad_dtype == torch.bfloat16)
+        if a.partials:
+            b.emit(nat.OP_GRAD_NORM, ints=(t.nchunks, bf16), ptrs=(a.chunks, a.partials))
+        # the piece table and its length also as operands: a grouped program checks its pointers there
+        b.emit(nat.OP_ADAMW, payload=a, ints=(st.bits, bf16, t.nchunks),
+               floats=(opt.learning_rate, opt.weight_decay), ptrs=(a.chunks,))
 
     # ------------------------------------------------------------------ execution
     def _sh(self):
@@ -463,8 +478,8 @@ class FusedProgram:
                 self.run_range(lo, hi)
 
     def set_lr(self, lr: float):
-        if self.rms_index is not None:
-            self.plan.set_float(self.rms_index, 0, float(lr))
+        if self.opt_index is not None:
+            self.plan.set_float(self.opt_index, 0, float(lr))  # RMSprop's and AdamW's first float
             self.plan.clear_graphs()
             self.graphs = {}
             self._bwd_graphs = None
@@ -697,7 +712,7 @@ class FusedStep:
         p.run_segment("bwd")
         st.reduce_to_root(m.arena.grad, p.stream)
         if "opt" in p.seg:
-            lo, hi = p.seg["opt"]  # [finite check] rmsprop | cast [flag reset]
+            lo, hi = p.seg["opt"]  # [finite check] [grad norm] update | cast [flag reset]
             if p.host_optimizer:
                 if st.rank == 0:
                     with torch.cuda.stream(p.stream):
@@ -705,8 +720,8 @@ class FusedStep:
                 cast_lo = lo
             else:
                 if st.rank == 0:
-                    p.run_range(lo, p.rms_index + 1, graph=False)
-                cast_lo = p.rms_index + 1
+                    p.run_range(lo, p.opt_index + 1, graph=False)
+                cast_lo = p.opt_index + 1
             st.broadcast_from_root(m.arena.data, p.stream)
             p.run_range(cast_lo, hi, graph=False)
         torch.cuda.current_stream(m.device).wait_stream(p.stream)
