@@ -9,7 +9,7 @@ struct OptChunk {
   const void* g;     // gradients, fp32 or bf16
   long long base;    // the piece's place in the flat state: a multiple of 64
   int n;             // elements, 1 .. the table's chunk size
-  int flags;         // bit 0: weight decay; bit 1: w and g may be read and written as vectors of 4
+  int flags;         // bit 0: weight decay; bit 1: w and g begin at multiples of 16 bytes
 };
 // Elements a workgroup takes at a time: OPT_CHUNK, and OPT_CHUNK_BIG in a table that has at least
 // OPT_MAX_GRID pieces of that size.  us for fp32 gradients, 32-bit states, 2048 / 4096: 2.2M weights 11.4 /

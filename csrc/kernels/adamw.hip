@@ -195,7 +195,8 @@ __device__ __forceinline__ void moments(F4& m, F4& v, const F4& g, float b1, flo
 }
 // The decay is subtracted, not multiplied as (1 - lr wd): that factor would keep few of lr wd's bits.
 // The quotient is a reciprocal (to one unit in its last place) and a product: 3 half steps of fp32 in
-// the update, which a weight's own rounding hides, for a third of a division's instructions.
+// the update, which a weight's own rounding hides, for a third of a division's instructions (8-bit states,
+// 7M weights: 23.3 -> 21.1 us).  eps is a normal number, and so is what is inverted.
 __device__ __forceinline__ void update(F4& w, const F4& m, const F4& root, float lr_wd, const Hyper& h) {
 #pragma unroll
   for (int j = 0; j < 4; ++j)

@@ -201,6 +201,8 @@ class AdamW(Optimizer):
 
     def step(self, arena=None, lr=None, grad_scale: float = 1.0):
         arena = arena or self._arena
+        if arena is not self._arena:
+            raise ValueError("AdamW steps the arena that it is bound to")
         if self._should_skip(arena):
             return
         lr = self.learning_rate if lr is None else lr

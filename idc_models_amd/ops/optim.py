@@ -23,6 +23,7 @@ import torch
 from . import _native as nat
 from . import moments8
 
+_MIN, _MAX = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max
 _CHUNK = np.dtype([("w", "u8"), ("g", "u8"), ("base", "i8"), ("n", "i4"), ("flags", "i4")])
 
 
@@ -67,7 +68,7 @@ def chunk_table(sizes: Sequence[int], w_ptrs: Sequence[int], g_ptrs: Sequence[in
     room = (n + nat.OPT_BLOCK - 1) // nat.OPT_BLOCK * nat.OPT_BLOCK
     offsets = np.concatenate([[0], np.cumsum(room)])
     w, g = np.asarray(w_ptrs, dtype=np.uint64), np.asarray(g_ptrs, dtype=np.uint64)
-    vec = (w % 16 == 0) & (g % (4 * grad_bytes) == 0)
+    vec = (w % 16 == 0) & (g % 16 == 0)
     flags = np.asarray(decay, dtype=bool) * nat.OPT_DECAY + vec * nat.OPT_VEC
     count = (n + chunk - 1) // chunk
     of = np.repeat(np.arange(len(n)), count)  # the tensor of every piece
@@ -254,10 +255,12 @@ def check_adamw(lr: float, beta_1: float, beta_2: float, epsilon: float, weight_
     """Raises ValueError for hyperparameters an AdamW step cannot run with."""
     if not (0.0 <= beta_1 < 1.0 and 0.0 <= beta_2 < 1.0):
         raise ValueError(f"betas have to be in [0, 1): {beta_1}, {beta_2}")
-    if not (epsilon >= 0.0 and lr >= 0.0 and weight_decay >= 0.0 and clip_norm >= 0.0
-            and math.isfinite(epsilon + lr + weight_decay + clip_norm)):
-        raise ValueError("lr, epsilon, weight_decay and clip_norm have to be finite and not negative: "
-                         f"{lr}, {epsilon}, {weight_decay}, {clip_norm}")
+    if not (lr >= 0.0 and weight_decay >= 0.0 and clip_norm >= 0.0 and max(lr, weight_decay, clip_norm, epsilon) <= _MAX):
+        raise ValueError("lr, weight_decay and clip_norm have to be finite and not negative: "
+                         f"{lr}, {weight_decay}, {clip_norm}")
+    if not epsilon >= _MIN:
+        # without it, every weight whose gradients have all been zero would become 0 / 0
+        raise ValueError(f"epsilon has to be a positive fp32 number: {epsilon}")
 
 
 def set_adamw_args(a: "nat.AdamwArgs", table: TensorTable, state: AdamWState, lr: float, beta_1: float, beta_2: float,
@@ -289,6 +292,8 @@ def adamw_(table: TensorTable, state: AdamWState, lr: float, beta_1: float = 0.9
     is read back; a norm that is not finite makes every gradient NaN).  ``skip``: an int32 tensor on the device; if its
     first word is not zero the call changes nothing."""
     check_adamw(lr, beta_1, beta_2, epsilon, weight_decay, clip_norm)
+    if not abs(grad_scale) <= _MAX:
+        raise ValueError(f"grad_scale has to be finite: {grad_scale}")
     if table.params is None:
         raise ValueError("the table has no params")
     if state.numel != table.numel or state.device != table.device:

@@ -84,6 +84,8 @@ def test_skip_nonfinite_and_reset():
     arena.grad[3] = float("inf")
     opt.step()
     assert opt.skipped == 1 and all(torch.equal(a, b) for a, b in zip(before, [arena.data] + list(opt.state_tensors().values())))
+    with pytest.raises(ValueError, match="bound to"):
+        opt.step(small_arena()[0])
     opt.reset_state()
     assert all(int(t.abs().max() if t.dtype != torch.uint8 else t.max()) == 0 for t in opt.state_tensors().values())
 

@@ -26,7 +26,7 @@ def make(sizes, layout, grad_dtype=torch.float32, seed=0):
         gs.append(rand(n, seed=seed + 2 * i + 1, scale=10.0 ** (i % 5 - 3)).to(grad_dtype))
     if layout == "own":
         return [p.to(DEV) for p in ps], [g.to(DEV) for g in gs], None
-    gap = 0 if layout == "arena" else 1
+    gap = {"arena": 0, "odd": 1, "half": 4}[layout]  # "half": multiples of 8 bytes (bf16), or of 16
     offs, total = [], gap
     for n in sizes:
         offs.append(total)
@@ -143,7 +143,7 @@ def bounds_each(x, mantissa, r16, slack):
 SIZES = [[1], [3, 64, 65, 1], [2048], [2047, 0, 2049, 5], [4096 + 17, 63, 128], [1] * 70, [30011, 1025], [0, 0]]
 
 
-@pytest.mark.parametrize("layout", ["own", "arena", "odd"])
+@pytest.mark.parametrize("layout", ["own", "arena", "odd", "half"])
 @pytest.mark.parametrize("grad_dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("bits", [32, 8])
 def test_step_matches_the_formula(bits, grad_dtype, layout):
@@ -292,6 +292,56 @@ def test_values_that_are_not_finite():
             assert bool(torch.isnan(p).all()) and not math.isfinite(float(st.norm))
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_second_moment_that_leaves_fp32(bits):
+    """A square beyond fp32: the first moment stays finite, the weight keeps still in this step; an 8-bit
+    block reads as NaN from then on, by its second moment alone."""
+    p, g = rand(200, seed=4).to(DEV), rand(200, seed=5).to(DEV)
+    table, st = start([p], [g], bits, 3, [True])
+    assert bool(torch.isfinite(state_values(st)[1]).all())
+    g[70] = 1e25
+    check_step_fp32(p, g, table, st)
+    m, v = state_values(st)
+    assert bool(torch.isfinite(m).all()) and bool(torch.isfinite(p).all())
+    bad = (~torch.isfinite(v)).nonzero().flatten().tolist()
+    assert bad == ([70] if bits == 32 else list(range(64, 128)))
+
+
+def check_step_fp32(p, g, table, st):
+    """One step where the oracle's second moment has to leave fp32's range as fp32 does."""
+    from idc_models_amd.ops import optim
+    w0, _ = orc.place([p])
+    m0, v0 = state_values(st)
+    g0, _ = orc.place([g])
+    optim.adamw_(table, st, **HYPER)
+    g1 = torch.where(g0 > 1e20, torch.full_like(g0, 1e200), g0)
+    w1, *_, tw, _, _, _ = orc.step(w0, g1, m0, v0, int(st.step[0]), HYPER["lr"], 0.9, 0.999, 1e-7, 0.1, torch.ones_like(w0))
+    keep = g0 < 1e20
+    got, _ = orc.place([p])
+    orc.within(got[keep], w1[keep], tw[keep])
+    i = int((~keep).nonzero()[0])  # m / inf: only the decay is left
+    assert float(got[i]) == pytest.approx(float(w0[i]) * (1 - HYPER["lr"] * HYPER["weight_decay"]), rel=1e-6)
+
+
+def test_refused_calls():
+    from idc_models_amd.ops import optim
+    p, g = torch.zeros(100, device=DEV), torch.zeros(100, device=DEV)
+    table = optim.TensorTable([g], [p])
+    st = optim.AdamWState(table)
+    other = optim.AdamWState(optim.TensorTable([g.new_zeros(200)], [p.new_zeros(200)]))
+    norm_only = optim.TensorTable([g])
+    for call in (lambda: optim.adamw_(table, other, 1e-3), lambda: optim.adamw_(norm_only, st, 1e-3),
+                 lambda: optim.AdamWState(norm_only), lambda: optim.AdamWState(table, bits=4), lambda: st.decode(),
+                 lambda: optim.adamw_(table, st, math.nan), lambda: optim.adamw_(table, st, 1e-3, grad_scale=math.inf),
+                 lambda: optim.adamw_(table, st, 1e-3, skip=torch.zeros(1, device=DEV)),
+                 lambda: optim.adamw_(table, st, 1e-3, skip=torch.zeros(1, dtype=torch.int32)),
+                 lambda: optim.AdamWState(table, bits=8).decode(torch.float16),
+                 lambda: st.load_moments(st.m[:64], st.v)):
+        with pytest.raises(ValueError):
+            call()
+    assert int(st.step[0]) == 0
+
+
 def test_scale_borders_are_exact():
     """A block whose largest value is exactly a unit's largest code keeps that unit; the next number up
     takes the next one."""
@@ -374,7 +424,7 @@ def test_same_bits_every_time_and_on_another_stream():
 def test_global_norm(grad_dtype):
     from idc_models_amd.ops.optim import TensorTable, global_norm
     for sizes in ([1], [0], [3, 64, 0, 65], [2048 * 8], [2048 * 8 + 1], [2048 * 1500 + 5, 9, 1]):
-        for layout in ("own", "odd"):
+        for layout in ("own", "odd", "half"):
             _, grads, _ = make(sizes, layout, grad_dtype, seed=7)
             want = orc.norm(grads)
             got = global_norm(TensorTable(grads))
