@@ -443,19 +443,42 @@ __device__ __forceinline__ double chunk_squares(const OptChunk& k) {
   return s;
 }
 
-template <bool GB, bool LAST>
+template <bool GB>
 __global__ __launch_bounds__(TPB) void grad_norm_kernel(const OptChunk* chunks, int nchunks, double* partials,
-                                                        float* out, GroupArg ga) {
+                                                        GroupArg ga) {
   const long long go = goff(ga);
   chunks = gsh(chunks, go);
   partials = gsh(partials, go);
-  out = gsh(out, go);
   double s = 0.0;
   for (int c = blockIdx.x; c < nchunks; c += gridDim.x) s += chunk_squares<GB>(get_chunk(chunks + c, go));
   s = block_sum64(s);
+  if (threadIdx.x == 0) partials[blockIdx.x] = s;
+}
+
+// The norm of a small table in one launch: a wave takes a piece at a time.
+constexpr int ONE_TPB = 1024;
+template <bool GB>
+__global__ __launch_bounds__(ONE_TPB) void grad_norm_one_kernel(const OptChunk* chunks, int nchunks, float* out) {
+  __shared__ double part[ONE_TPB / 64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  double s = 0.0;
+  for (int c = wave; c < nchunks; c += ONE_TPB / 64) {
+    const OptChunk k = get_chunk(chunks + c, 0);
+    const bool vec = k.flags & OPT_VEC;
+    for (int e = lane * 4; e < k.n; e += 1024) {
+      F4 g[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) g[j] = edge_g<GB>(k.g, e + j * 256, k.n, vec);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s += sum4(g[j]);
+    }
+  }
+  s = wave_sum64(s);
+  if (lane == 0) part[wave] = s;
+  __syncthreads();
   if (threadIdx.x == 0) {
-    if (LAST) *out = (float)sqrt(s);
-    else partials[blockIdx.x] = s;
+    for (int i = 1; i < ONE_TPB / 64; ++i) s += part[i];
+    *out = (float)sqrt(s);
   }
 }
 
@@ -533,7 +556,7 @@ hipError_t adamw(const AdamwArgs& a, int bits, int g_bf16, hipStream_t st) {
   if ((bits != 8 && bits != 32) || (a.chunk != OPT_CHUNK && a.chunk != OPT_CHUNK_BIG) || !a.step || a.nchunks < 0 ||
       !a.norm || (a.nchunks && !(a.chunks && a.m && a.v)) || (bits == 8 && a.nchunks && !a.scales))
     return hipErrorInvalidValue;
-  if (a.clip > 0.f && (a.partials ? a.npartials < 1 || a.npartials > OPT_MAX_GRID : a.nchunks > OPT_NORM_ONE))
+  if (a.clip > 0.f && (a.partials ? a.npartials < 1 || a.npartials > OPT_MAX_GRID : a.nchunks > OPT_OWN_SUM))
     return hipErrorInvalidValue;
   if (bits == 8) {
     if (g_bf16) launch_adamw<8, true>(a, st);
@@ -548,27 +571,22 @@ hipError_t adamw(const AdamwArgs& a, int bits, int g_bf16, hipStream_t st) {
 hipError_t grad_norm_partials(const OptChunk* chunks, int nchunks, int g_bf16, double* partials, hipStream_t st) {
   if (nchunks < 0 || (nchunks && !chunks) || !partials) return hipErrorInvalidValue;
   const dim3 grid = ggrid(opt_grid(nchunks));
-  if (g_bf16) hipLaunchKernelGGL((grad_norm_kernel<true, false>), grid, dim3(TPB), 0, st, chunks, nchunks, partials,
-                                 (float*)nullptr, garg());
-  else hipLaunchKernelGGL((grad_norm_kernel<false, false>), grid, dim3(TPB), 0, st, chunks, nchunks, partials,
-                          (float*)nullptr, garg());
+  if (g_bf16) hipLaunchKernelGGL(grad_norm_kernel<true>, grid, dim3(TPB), 0, st, chunks, nchunks, partials, garg());
+  else hipLaunchKernelGGL(grad_norm_kernel<false>, grid, dim3(TPB), 0, st, chunks, nchunks, partials, garg());
   return hipGetLastError();
 }
 
 hipError_t grad_norm(const OptChunk* chunks, int nchunks, int g_bf16, double* partials, float* out, hipStream_t st) {
   if (nchunks < 0 || (nchunks && !chunks) || (nchunks > OPT_NORM_ONE && !partials) || !out) return hipErrorInvalidValue;
   if (nchunks <= OPT_NORM_ONE) {
-    if (g_bf16) hipLaunchKernelGGL((grad_norm_kernel<true, true>), dim3(1), dim3(TPB), 0, st, chunks, nchunks,
-                                   partials, out, GroupArg{0, 1, 0});
-    else hipLaunchKernelGGL((grad_norm_kernel<false, true>), dim3(1), dim3(TPB), 0, st, chunks, nchunks, partials,
-                            out, GroupArg{0, 1, 0});
+    if (g_bf16) hipLaunchKernelGGL(grad_norm_one_kernel<true>, dim3(1), dim3(ONE_TPB), 0, st, chunks, nchunks, out);
+    else hipLaunchKernelGGL(grad_norm_one_kernel<false>, dim3(1), dim3(ONE_TPB), 0, st, chunks, nchunks, out);
     return hipGetLastError();
   }
   const int grid = opt_grid(nchunks);
-  if (g_bf16) hipLaunchKernelGGL((grad_norm_kernel<true, false>), dim3(grid), dim3(TPB), 0, st, chunks, nchunks,
-                                 partials, (float*)nullptr, GroupArg{0, 1, 0});
-  else hipLaunchKernelGGL((grad_norm_kernel<false, false>), dim3(grid), dim3(TPB), 0, st, chunks, nchunks, partials,
-                          (float*)nullptr, GroupArg{0, 1, 0});
+  const GroupArg alone{0, 1, 0};
+  if (g_bf16) hipLaunchKernelGGL(grad_norm_kernel<true>, dim3(grid), dim3(TPB), 0, st, chunks, nchunks, partials, alone);
+  else hipLaunchKernelGGL(grad_norm_kernel<false>, dim3(grid), dim3(TPB), 0, st, chunks, nchunks, partials, alone);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(norm_of_partials_kernel, dim3(1), dim3(TPB), 0, st, partials, grid, out);

@@ -1160,6 +1160,7 @@ PYBIND11_MODULE(_idc_native, m) {
   m.attr("OPT_CHUNK") = OPT_CHUNK;
   m.attr("OPT_CHUNK_BIG") = OPT_CHUNK_BIG;
   m.attr("OPT_NORM_ONE") = OPT_NORM_ONE;
+  m.attr("OPT_OWN_SUM") = OPT_OWN_SUM;
   m.attr("OPT_MAX_GRID") = OPT_MAX_GRID;
   m.attr("OPT_BLOCK") = OPT_BLOCK;
   m.attr("OP_ADAMW") = (int)OP_ADAMW;

@@ -221,7 +221,7 @@ class AdamW(Optimizer):
             norm = arena.grad.double().square().sum().sqrt().float() * abs(grad_scale)
             if not bool(norm <= self.clip_norm):
                 g = g * (self.clip_norm / norm if bool(torch.isfinite(norm)) else float("nan"))
-        m, v = self._values()
+        m, v = self.moments()
         # each product and sum rounded by itself, as the kernel does: the same bits, the same codes
         m = self.beta_1 * m + (1.0 - self.beta_1) * g
         v = self.beta_2 * v + (1.0 - self.beta_2) * (g * g)
@@ -239,8 +239,10 @@ class AdamW(Optimizer):
             self.m[:], self.scales[:, 0] = moments8.encode(m, moments8.M_BITS, low)
             self.v[:], self.scales[:, 1] = moments8.encode(root, moments8.ROOT_BITS, high)
 
-    def _values(self):
-        """Both moments in fp32 (a CPU state, or a checkpoint's tensors)."""
+    def moments(self):
+        """First and second moments in fp32, by place in the arena (of a 32-bit state its own tensors)."""
+        if self.state is not None:
+            return self.state.moments()
         return _moment_values({"m": self.m, "v": self.v, "scales": self.scales})
 
     def state_tensors(self):

@@ -216,7 +216,8 @@ class AdamwArgs(C.Structure):
                [("nchunks", ci), ("npartials", ci), ("chunk", ci), ("pad", ci)]
 
 
-OPT_CHUNK, OPT_CHUNK_BIG, OPT_MAX_GRID, OPT_BLOCK, OPT_NORM_ONE = 2048, 4096, 1024, 64, 8  # csrc/kernels/adamw.h
+# csrc/kernels/adamw.h
+OPT_CHUNK, OPT_CHUNK_BIG, OPT_MAX_GRID, OPT_BLOCK, OPT_OWN_SUM, OPT_NORM_ONE = 2048, 4096, 1024, 64, 8, 32
 OPT_DECAY, OPT_VEC = 1, 2
 
 
@@ -263,8 +264,8 @@ def _verify(ext):
             or ext.OP_DENSE_INFER != OP_DENSE_INFER:
         raise RuntimeError("native op-kind table drifted (OP_DENSE_STAGE / OP_MB_CHAIN)")
     if (ext.OP_ADAMW, ext.OP_GRAD_NORM) != (OP_ADAMW, OP_GRAD_NORM) \
-            or (ext.OPT_CHUNK, ext.OPT_CHUNK_BIG, ext.OPT_MAX_GRID, ext.OPT_BLOCK, ext.OPT_NORM_ONE) \
-            != (OPT_CHUNK, OPT_CHUNK_BIG, OPT_MAX_GRID, OPT_BLOCK, OPT_NORM_ONE):
+            or (ext.OPT_CHUNK, ext.OPT_CHUNK_BIG, ext.OPT_MAX_GRID, ext.OPT_BLOCK, ext.OPT_OWN_SUM, ext.OPT_NORM_ONE) \
+            != (OPT_CHUNK, OPT_CHUNK_BIG, OPT_MAX_GRID, OPT_BLOCK, OPT_OWN_SUM, OPT_NORM_ONE):
         raise RuntimeError("native multi-tensor optimizer constants drifted")
     sizes = ext.struct_sizes()
     for name, cls in _STRUCTS.items():

@@ -272,7 +272,7 @@ def set_adamw_args(a: "nat.AdamwArgs", table: TensorTable, state: AdamWState, lr
     a.log_b2 = math.log(beta_2) if beta_2 else -math.inf
     a.lr, a.eps, a.lr_wd = lr, epsilon, lr * weight_decay
     a.grad_scale, a.clip = grad_scale, clip_norm
-    if clip_norm and table.nchunks > nat.OPT_NORM_ONE:  # grad_norm's partial sums; else the step sums by itself
+    if clip_norm and table.nchunks > nat.OPT_OWN_SUM:  # grad_norm's partial sums; else the step sums by itself
         a.partials, a.npartials = state.partials.data_ptr(), min(table.nchunks, nat.OPT_MAX_GRID)
     else:
         a.partials, a.npartials = 0, 0

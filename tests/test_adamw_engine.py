@@ -107,7 +107,7 @@ def test_checkpoints_of_either_width(tmp_path, width):
     b = tiny(AdamW(1e-3, state_bits=width[1]), seed=3)
     b.load_checkpoint(path)
     assert b.optimizer.iterations == 4 and bool((b.optimizer.steps == 4).all())
-    (ma, va), (mb, vb) = a.optimizer._values(), b.optimizer._values()
+    (ma, va), (mb, vb) = a.optimizer.moments(), b.optimizer.moments()
     if width in ((32, 32), (8, 8), (8, 32)):  # codes are fp32 values
         assert torch.equal(ma, mb) and torch.equal(va, vb)
         return

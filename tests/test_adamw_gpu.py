@@ -423,7 +423,7 @@ def test_same_bits_every_time_and_on_another_stream():
 @pytest.mark.parametrize("grad_dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
 def test_global_norm(grad_dtype):
     from idc_models_amd.ops.optim import TensorTable, global_norm
-    for sizes in ([1], [0], [3, 64, 0, 65], [2048 * 8], [2048 * 8 + 1], [2048 * 1500 + 5, 9, 1]):
+    for sizes in ([1], [0], [3, 64, 0, 65], [2048 * 8], [2048 * 32 - 3], [2048 * 32 + 1], [5] * 32, [77] * 33, [2048 * 1500 + 5, 9, 1]):
         for layout in ("own", "odd", "half"):
             _, grads, _ = make(sizes, layout, grad_dtype, seed=7)
             want = orc.norm(grads)

@@ -156,6 +156,8 @@ def test_checkpoint_resumes_on_the_gpu(tmp_path, width):
     assert torch.equal(a.arena.data, b.arena.data) and bool((b.optimizer.steps == 2).all())
     ma, va = values(a.optimizer)
     mb, vb = values(b.optimizer)
+    for have, want in zip(b.optimizer.moments(), (mb, vb)):  # the kernel's decoding: r * r in fp32
+        assert bool(((have.double().cpu() - want).abs() <= orc.U * want.abs() + 2.0 ** -149).all())
     if width[1] == 32 or width[0] == 8:
         assert torch.equal(ma, mb) and torch.equal(va, vb)
     else:
