@@ -289,7 +289,8 @@ def adamw_(table: TensorTable, state: AdamWState, lr: float, beta_1: float = 0.9
         w -= lr*weight_decay*w + lr*sqrt(1-beta_2^t)/(1-beta_1^t) * m/(sqrt(v)+epsilon)
 
     ``clip_norm`` > 0 scales g down to that global norm (one launch more for all but small tables, nothing
-    is read back; a norm that is not finite makes every gradient NaN).  ``skip``: an int32 tensor on the device; if its
+    is read back; a norm that is not finite makes every gradient NaN).  The numbers are arguments of the
+    launch: a captured call keeps those it was captured with, and counts its steps on the device.  ``skip``: an int32 tensor on the device; if its
     first word is not zero the call changes nothing."""
     check_adamw(lr, beta_1, beta_2, epsilon, weight_decay, clip_norm)
     if not abs(grad_scale) <= _MAX:

@@ -354,10 +354,10 @@ class FusedProgram:
                           reset_tickets=b.reset_tickets, slab_floats=b.SLAB_FLOATS)
         b.reset_tickets()  # split-K tickets count modulo the op's split: start every op aligned
 
-    @staticmethod
-    def _emit_adamw(b, opt, grad_scale: float, skip: int, hostflag: int):
+    def _emit_adamw(self, b, opt, grad_scale: float, skip: int, hostflag: int):
         from ..ops import optim
-        t, st = opt.table, opt.state
+        # the plan holds addresses only: the optimizer may be bound to another model while it lives
+        t, st = self._opt_keep = opt.table, opt.state
         a = optim.set_adamw_args(nat.AdamwArgs.from_buffer_copy(st._args), t, st, opt.learning_rate, opt.beta_1,
                                  opt.beta_2, opt.epsilon, opt.weight_decay, grad_scale, opt.clip_norm, skip, hostflag)
         bf16 = int(t.grad_dtype == torch.bfloat16)
