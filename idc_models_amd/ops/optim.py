@@ -255,9 +255,10 @@ def check_adamw(lr: float, beta_1: float, beta_2: float, epsilon: float, weight_
     """Raises ValueError for hyperparameters an AdamW step cannot run with."""
     if not (0.0 <= beta_1 < 1.0 and 0.0 <= beta_2 < 1.0):
         raise ValueError(f"betas have to be in [0, 1): {beta_1}, {beta_2}")
-    if not (lr >= 0.0 and weight_decay >= 0.0 and clip_norm >= 0.0 and max(lr, weight_decay, clip_norm, epsilon) <= _MAX):
-        raise ValueError("lr, weight_decay and clip_norm have to be finite and not negative: "
-                         f"{lr}, {weight_decay}, {clip_norm}")
+    if not (lr >= 0.0 and weight_decay >= 0.0 and max(lr, weight_decay, lr * weight_decay, epsilon) <= _MAX):
+        raise ValueError(f"lr and weight_decay have to be finite and not negative: {lr}, {weight_decay}")
+    if not (clip_norm == 0.0 or _MIN <= clip_norm <= _MAX):
+        raise ValueError(f"clip_norm has to be 0 (no clipping) or a positive fp32 number: {clip_norm}")
     if not epsilon >= _MIN:
         # without it, every weight whose gradients have all been zero would become 0 / 0
         raise ValueError(f"epsilon has to be a positive fp32 number: {epsilon}")
@@ -289,9 +290,9 @@ def adamw_(table: TensorTable, state: AdamWState, lr: float, beta_1: float = 0.9
         w -= lr*weight_decay*w + lr*sqrt(1-beta_2^t)/(1-beta_1^t) * m/(sqrt(v)+epsilon)
 
     ``clip_norm`` > 0 scales g down to that global norm (one launch more for all but small tables, nothing
-    is read back; a norm that is not finite makes every gradient NaN).  The numbers are arguments of the
-    launch: a captured call keeps those it was captured with, and counts its steps on the device.  ``skip``: an int32 tensor on the device; if its
-    first word is not zero the call changes nothing."""
+    is read back; a norm that is not finite makes every gradient NaN).  ``skip``: an int32 tensor on the
+    device; if its first word is not zero the call changes nothing.  The numbers are arguments of the
+    launch: a captured call keeps those it was captured with, and counts its steps on the device."""
     check_adamw(lr, beta_1, beta_2, epsilon, weight_decay, clip_norm)
     if not abs(grad_scale) <= _MAX:
         raise ValueError(f"grad_scale has to be finite: {grad_scale}")
@@ -313,7 +314,8 @@ def adamw_(table: TensorTable, state: AdamWState, lr: float, beta_1: float = 0.9
 
 def global_norm(table: TensorTable) -> torch.Tensor:
     """sqrt of the sum of the squares of all the table's gradients: an fp32 tensor without axes.
-    Sums in fp64 in a fixed order (the same bits every time)."""
+    Sums in a fixed order (the same bits every time), in fp64; of bf16 gradients up to 16 squares, exact
+    in fp32, are summed there first, where none of them leaves its range."""
     dev = table.device
     many = table.nchunks > nat.OPT_NORM_ONE
     partials = torch.empty(nat.OPT_MAX_GRID, dtype=torch.float64, device=dev) if many else None

@@ -53,7 +53,8 @@ def test_refused_hyperparameters():
     ok = dict(lr=1e-3, beta_1=0.9, beta_2=0.999, epsilon=1e-7, weight_decay=0.0, clip_norm=0.0)
     optim.check_adamw(**ok)
     for k, v in (("beta_1", 1.0), ("beta_1", -0.1), ("beta_2", 1.0), ("beta_2", math.nan), ("lr", -1.0), ("lr", math.inf),
-                 ("lr", math.nan), ("epsilon", -1e-9), ("epsilon", 0.0), ("epsilon", 1e-39), ("epsilon", math.nan), ("epsilon", 1e39), ("weight_decay", -1.0), ("clip_norm", -1.0), ("clip_norm", math.inf)):
+                 ("lr", math.nan), ("epsilon", -1e-9), ("epsilon", 0.0), ("epsilon", 1e-39), ("epsilon", math.nan), ("epsilon", 1e39), ("weight_decay", -1.0), ("clip_norm", -1.0), ("clip_norm", math.inf), ("clip_norm", 1e-40),
+                 ("clip_norm", math.nan), ("lr", 1e39)):
         with pytest.raises(ValueError):
             optim.check_adamw(**dict(ok, **{k: v}))
 
