@@ -177,3 +177,25 @@ def test_cli_trains_with_adamw(tmp_path, capsys):
                    "steps_per_epoch: 1\nplot: false\noptimizer_args: {state_bits: 8, global_clipnorm: 1.0, decay: kernels}\n")
     main(["dist", "mobile", str(tmp_path), "--synthetic", "--strategy", "one", "--config", str(cfg), "--optimizer", "adamw"])
     assert "Number of layers" in capsys.readouterr().out
+
+
+def _replica(rank, world, kind, bits):
+    from idc_models_amd.data import synthetic_dataset
+    from idc_models_amd.parallel import CentralStorageStrategy, MirroredStrategy
+    st = (MirroredStrategy if kind == "mirrored" else CentralStorageStrategy)(backend="gloo")
+    torch.manual_seed(rank)  # dropout differs, what is reduced is one gradient
+    m = Model(build_model("tinycnn", seed=3), st)
+    m.compile(AdamW(1e-2, global_clipnorm=0.1, state_bits=bits), "binary_crossentropy", ["accuracy"], backend="eager")
+    m.fit(synthetic_dataset(64, (10, 10, 3), seed=11).batch(16, drop_remainder=True), epochs=2, verbose=0)
+    return m.arena.data.numpy().copy(), {k: t.numpy().copy() for k, t in m.optimizer.state_tensors().items()}
+
+
+@pytest.mark.parametrize("kind,bits", [("mirrored", 8), ("mirrored", 32), ("central", 8)])
+def test_replicas_stay_the_same(kind, bits):
+    from idc_models_amd.parallel.launch import spawn
+    (w0, s0), (w1, s1) = spawn(_replica, 2, (kind, bits))
+    assert (w0 == w1).all() and (s0["step"] == 8).all()
+    if kind == "mirrored":
+        assert all((s0[k] == s1[k]).all() for k in s0)
+    else:  # rank 0 owns the state
+        assert (s1["step"] == 0).all() and (s1["m"] == 0).all() and (s0["m"] != 0).any()
