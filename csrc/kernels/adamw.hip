@@ -5,8 +5,10 @@
 //   m <- b1 m + (1 - b1) s g;  v <- b2 v + (1 - b2) (s g)^2
 //   w <- w - lr wd w - lr sqrt(1 - b2^t) / (1 - b1^t) * m / (sqrt(v) + eps)
 //
-// A launch walks over a table of pieces (OptChunk) of at most OPT_CHUNK elements, so tensors of any
-// size share it; every tensor starts at a multiple of 64 in the flat state.
+// A launch walks over a table of pieces (OptChunk) of at most 2048 or 4096 elements, so tensors of any
+// size share it; every tensor starts at a multiple of 64 in the flat state.  Memory bounds it: 24 bytes a
+// weight and the gradient's 4 or 2 (32-bit states), or 12 and the gradient's (8-bit); 120M weights with bf16
+// gradients take 518 us on the device (6.0 TB/s) and 268 us (6.3 TB/s).
 //
 // The step counter is OPT_MAX_GRID equal words: a workgroup reads its own and writes it (and those
 // of the workgroups this launch does not have) at its end, so a captured launch counts its replays
@@ -411,7 +413,7 @@ template <bool GB, int ROWS>
 __device__ __forceinline__ double full_squares(const OptChunk& k) {
   double s = 0.0;
   if constexpr (GB) {
-    // Converting to double costs more than reading a bf16 (120M: 72 us against 60).  Its square is
+    // Converting to double costs more than reading a bf16 (120M: 72 us, this way 40).  Its square is
     // exact in fp32, so a thread's squares of this piece are summed there, unless their sum is so small or
     // large that some may have left fp32's range.
     uint4 x[ROWS / 2];
