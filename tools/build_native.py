@@ -72,15 +72,32 @@ def _headers():
     return hs
 
 
-def _compile(src: str, extra) -> str:
+def _make(cmd, out: str, deps, what: str) -> None:
+    """Runs ``cmd -o out`` unless that very command has made ``out`` since ``deps`` last changed: the
+    object directory keeps the command of every output (other flags are another output)."""
+    record = os.path.join(BUILD, os.path.basename(out) + ".cmd")
+    line = "\n".join(cmd)
+    if os.path.exists(record) and os.path.exists(out) and \
+            os.path.getmtime(out) >= max(os.path.getmtime(d) for d in deps):
+        with open(record) as f:
+            if f.read() == line:
+                return
+    r = subprocess.run(cmd + ["-o", out + ".tmp"], capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{what} failed:\n{r.stderr[-6000:]}")
+    if os.path.exists(record):
+        os.remove(record)  # never beside an output that it does not describe
+    os.replace(out + ".tmp", out)
+    with open(record, "w") as f:
+        f.write(line)
+
+
+def _compile(src: str) -> str:
     import pybind11
 
     s = os.path.join(CSRC, src)
     o = os.path.join(BUILD, src.replace("/", "_") + ".o")
-    newest_dep = max([os.path.getmtime(s)] + [os.path.getmtime(h) for h in _headers()])
-    if os.path.exists(o) and os.path.getmtime(o) >= newest_dep and not extra.get("force"):
-        return o
-    cmd = [HIPCC, f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-c", s, "-o", o,
+    cmd = [HIPCC, f"--offload-arch={ARCH}", "-O3", "-std=c++17", "-fPIC", "-c", s,
            f"-I{pybind11.get_include()}", f"-I{sysconfig.get_paths()['include']}",
            "-Wno-unused-result", "-Wno-unused-variable",
            # no packed fp32 arithmetic (v_pk_mul_f32 and its like, which -O3 forms by itself): some of
@@ -96,9 +113,7 @@ def _compile(src: str, extra) -> str:
         cmd += ["-mllvm", "-amdgpu-mfma-vgpr-form"]
     if src.endswith(".cpp"):
         cmd += ["-x", "hip"]
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if r.returncode != 0:
-        raise RuntimeError(f"hipcc failed for {src}:\n{r.stderr[-6000:]}")
+    _make(cmd, o, [s] + _headers(), f"hipcc for {src}")
     return o
 
 
@@ -238,15 +253,9 @@ def build(clean: bool = False, jobs: int = 8, verbose: bool = True) -> str:
         shutil.rmtree(BUILD)
     os.makedirs(BUILD, exist_ok=True)
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
-        objs = list(ex.map(lambda s: _compile(s, {}), SOURCES))
+        objs = list(ex.map(_compile, SOURCES))
     out = ext_path()
-    if not os.path.exists(out) or os.path.getmtime(out) < max(os.path.getmtime(o) for o in objs):
-        tmp = out + ".tmp"
-        cmd = [HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", tmp] + objs + LINK_LIBS
-        r = subprocess.run(cmd, capture_output=True, text=True)
-        if r.returncode != 0:
-            raise RuntimeError(f"link failed:\n{r.stderr[-4000:]}")
-        os.replace(tmp, out)
+    _make([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC"] + objs + LINK_LIBS, out, objs, "link")
     if verbose:
         print(f"[build_native] {out}")
     return out
