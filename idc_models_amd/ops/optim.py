@@ -55,6 +55,22 @@ def _span(t: torch.Tensor) -> Tuple[int, int]:
     return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
 
 
+class _Held:
+    """The memory at addresses that are read once.  A tensor object does not hold it: ``p.data = x`` (and what
+    does that: ``Module.to``, the arena that ``Model.compile`` makes) gives the same object other storage and
+    frees the first one.  So an alias of each tensor is kept, and ``moved`` says whether one of the objects
+    lies elsewhere by now."""
+
+    def __init__(self, tensors: Sequence[torch.Tensor]):
+        self.tensors = list(tensors)
+        self.aliases = [t.detach() for t in self.tensors]
+        self.at, self.every = [t.data_ptr() for t in self.tensors], list(range(len(self.tensors)))
+
+    def moved(self) -> bool:
+        # one call into torch: 0.1 us for a tensor, 16 for 600 (data_ptr() in Python: 0.13 and 24)
+        return bool(self.every) and not torch._C._tensors_data_ptrs_at_indices_equal(self.tensors, self.at, self.every)
+
+
 def chunk_size(sizes: Sequence[int]) -> int:
     """Elements of a full piece of a table (csrc/kernels/adamw.h)."""
     return nat.OPT_CHUNK_BIG if sum(sizes) >= nat.OPT_MAX_GRID * nat.OPT_CHUNK_BIG else nat.OPT_CHUNK
@@ -87,8 +103,11 @@ class TensorTable:
     the fp32 weights they belong to.
 
     The addresses are read here once: gradients have to be accumulated in place afterwards, as an
-    arena's are.  A weight and its gradient have the same shape and the same order of axes in memory,
-    without gaps.  Empty tensors are fine.  ``decay``: which weights decay (default: all)."""
+    arena's are, and weights have to keep their storage.  Where it is replaced (``p.data = x``,
+    ``Module.to``, ``Model.compile``, which moves a model's weights into an arena), a new table is needed: ``adamw_``
+    refuses weights that are Parameters or require a gradient, ``check`` any tensor.  The table keeps the memory
+    alive.  A weight and its gradient have the same shape and the same order of axes in memory, without
+    gaps.  Empty tensors are fine.  ``decay``: which weights decay (default: all)."""
 
     def __init__(self, grads: Sequence[torch.Tensor], params: Optional[Sequence[torch.Tensor]] = None,
                  decay: Optional[Sequence[bool]] = None):
@@ -133,6 +152,8 @@ class TensorTable:
         if self.device.type != "cuda":
             raise ValueError("TensorTable needs tensors on a GPU")
         self.grads, self.params = grads, params
+        self._all = _Held(every)
+        self._leaves = _Held([p for p in params or [] if p.requires_grad or isinstance(p, torch.nn.Parameter)])
         sizes = [g.numel() for g in grads]
         self.chunk = chunk_size(sizes)
         pieces, offsets, self.numel = chunk_table(
@@ -145,6 +166,11 @@ class TensorTable:
         host = torch.from_numpy(pieces.view(np.uint8)) if self.nchunks else torch.zeros(1, dtype=torch.uint8)
         self.chunks = host.to(self.device)
         self._bf16 = int(self.grad_dtype == torch.bfloat16)
+
+    def check(self) -> None:
+        """Raises ValueError if any of the tensors has other storage than when the table was made."""
+        if self._all.moved():
+            raise ValueError("a tensor has other storage than when the table was made")
 
     def split(self, flat: torch.Tensor):
         """Views of a flat state tensor in the shapes of the table's contiguous tensors (others: flat
@@ -300,6 +326,8 @@ def adamw_(table: TensorTable, state: AdamWState, lr: float, beta_1: float = 0.9
         raise ValueError("the table has no params")
     if state.numel != table.numel or state.device != table.device:
         raise ValueError("the state was made for another table")
+    if table._leaves.moved():
+        raise ValueError("a weight has other storage than when the table was made")
     if skip is not None and (skip.dtype != torch.int32 or skip.device != table.device or not skip.numel()):
         raise ValueError("skip has to be an int32 tensor on the tensors' device")
     a = set_adamw_args(state._args, table, state, lr, beta_1, beta_2, epsilon, weight_decay, grad_scale, clip_norm,

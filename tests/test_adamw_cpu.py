@@ -143,3 +143,28 @@ def test_block_with_a_value_that_is_not_finite():
         v = moments8.decode(codes, scales, moments8.M_BITS)
         assert bool(torch.isnan(v[64:128]).all()) and bool((v[:64] == 1).all()) and bool((v[128:] == 1).all())
         assert bool((codes[64:128] == 0).all())
+
+
+def test_memory_at_held_addresses():
+    """Replacing a tensor's storage leaves the memory of the first one alive, and is seen."""
+    p, q = torch.nn.Parameter(torch.ones(1000)), torch.zeros(10)
+    at = p.data_ptr()
+    held = optim._Held([q, p])
+    assert not held.moved() and not optim._Held([]).moved()
+    with torch.no_grad():
+        p.add_(1.0)
+        p.grad = torch.zeros(1000)
+    assert not held.moved()
+    p.data = torch.full((1000,), 5.0)
+    assert held.moved()
+    others = [torch.full((1000,), 7.0) for _ in range(20)]  # none of them gets the first storage
+    assert held.aliases[1].data_ptr() == at and bool((held.aliases[1] == 2.0).all())
+    assert all(t.data_ptr() != at for t in others)
+    p.data = held.aliases[1]
+    assert not held.moved()
+    net = torch.nn.Linear(3, 4)
+    held = optim._Held(list(net.parameters()))
+    net.to(torch.float32)
+    assert not held.moved()
+    net.to(torch.float64)
+    assert held.moved()

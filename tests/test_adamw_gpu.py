@@ -490,3 +490,43 @@ def test_places_beyond_32_bits():
     assert float(p0[-1]) == pytest.approx(-HYPER["lr"], rel=1e-5) and float(p0[:-1].abs().max()) == 0.0
     n = optim.global_norm(table)
     assert float(n) == pytest.approx(math.sqrt(1.0 + float(g.square().sum())), rel=1e-6)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_weights_whose_storage_is_replaced(bits):
+    """A table over Parameters that an arena (or p.data = x) moves elsewhere: the step is refused and
+    changes nothing, neither the weights nor memory that other tensors have got since."""
+    from idc_models_amd.engine import ParamArena
+    from idc_models_amd.ops import optim
+    ps = [torch.nn.Parameter(rand(5000, seed=i).to(DEV)) for i in range(3)]
+    gs = [rand(5000, seed=10 + i).to(DEV) for i in range(3)]
+    table = optim.TensorTable(gs, ps)
+    st = optim.AdamWState(table, bits=bits)
+    optim.adamw_(table, st, **HYPER)  # in place: fine
+    table.check()
+    arena = ParamArena(ps)
+    before = [p.detach().clone() for p in ps]
+    others = [torch.full((5000,), 7.0, device=DEV) for _ in range(50)]
+    for _ in range(2):
+        with pytest.raises(ValueError, match="other storage"):
+            optim.adamw_(table, st, **HYPER)
+    with pytest.raises(ValueError, match="other storage"):
+        table.check()
+    torch.cuda.synchronize()
+    assert int(st.step[0]) == 1 and all(torch.equal(p, b) for p, b in zip(ps, before))
+    assert all(bool((o == 7.0).all()) for o in others)
+    table = optim.TensorTable([arena.grad_of(p) for p in ps], ps)  # a new table takes them where they are
+    optim.adamw_(table, st, **HYPER)
+    assert int(st.step[0]) == 2
+    # tensors that autograd does not know: the memory stays the table's own, check() sees the change
+    w, g = rand(3000, seed=1).to(DEV), rand(3000, seed=2).to(DEV)
+    table = optim.TensorTable([g], [w])
+    st = optim.AdamWState(table, bits=bits)
+    g.data = torch.zeros(3000, device=DEV)
+    with pytest.raises(ValueError, match="other storage"):
+        table.check()
+    w.data = torch.zeros(3000, device=DEV)
+    others = [torch.full((3000,), 7.0, device=DEV) for _ in range(50)]
+    optim.adamw_(table, st, **HYPER)
+    torch.cuda.synchronize()
+    assert all(bool((o == 7.0).all()) for o in others) and float(w.abs().max()) == 0.0
