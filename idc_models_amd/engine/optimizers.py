@@ -220,7 +220,8 @@ class AdamW(Optimizer):
         if self.clip_norm:
             norm = arena.grad.double().square().sum().sqrt().float() * abs(grad_scale)
             if not bool(norm <= self.clip_norm):
-                g = g * (self.clip_norm / norm if bool(torch.isfinite(norm)) else float("nan"))
+                # a quotient of two tensors: of a number and a tensor torch makes a reciprocal and a product
+                g = g * (torch.full_like(norm, self.clip_norm) / norm if bool(torch.isfinite(norm)) else float("nan"))
         m, v = self.moments()
         # each product and sum rounded by itself, as the kernel does: the same bits, the same codes
         m = self.beta_1 * m + (1.0 - self.beta_1) * g

@@ -199,3 +199,21 @@ def test_replicas_stay_the_same(kind, bits):
         assert all((s0[k] == s1[k]).all() for k in s0)
     else:  # rank 0 owns the state
         assert (s1["step"] == 0).all() and (s1["m"] == 0).all() and (s0["m"] != 0).any()
+
+
+def test_clipped_gradients_take_one_quotient():
+    """The factor of clipped gradients is clip / norm rounded once, as the GPU's: the first step's moments are
+    bits of (1 - beta_1) * (g * factor)."""
+    import numpy as np
+    f = np.float32
+    for seed in range(40):
+        g = torch.Generator().manual_seed(seed)
+        arena = ParamArena([torch.nn.Parameter(torch.randn(50, 7, generator=g))])
+        arena.grad.copy_(torch.randn(arena.numel, generator=g) * 3)
+        opt = AdamW(1e-2, global_clipnorm=0.7)
+        opt.bind(arena)
+        opt.step(grad_scale=0.3)
+        grad = arena.grad.numpy()
+        norm = f(np.sqrt(np.square(grad.astype(np.float64)).sum())) * f(0.3)
+        want = f(0.1) * ((grad * f(0.3)) * (f(0.7) / norm))
+        assert want.dtype == f and (opt.m.numpy() == want).all(), seed

@@ -209,3 +209,25 @@ def test_batched_clients_match_sequential(monkeypatch, bits):
         assert torch.equal(a, b), float((a - b).abs().max())
         assert all(torch.equal(sa.optimizer_state[k], sb.optimizer_state[k]) for k in sa.optimizer_state)
         assert int(sa.optimizer_state["step"][0]) == rounds
+
+
+@pytest.mark.parametrize("clip", [0.7, 0.013, 3.1])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_cpu_and_gpu_states_are_the_same_bits_when_clipped(bits, clip):
+    """Clip norms that are no powers of two, the gradients' norm above and below them; a table that its step sums
+    by itself, and one with partial sums."""
+    from idc_models_amd.engine import AdamW, ParamArena
+    for shapes in ([(9, 11), (11,)], [(200, 300), (300,), (1,)]):
+        g = torch.Generator().manual_seed(6)
+        init = [torch.randn(*s, generator=g) for s in shapes]
+        arenas = [ParamArena([torch.nn.Parameter(t.clone().to(d)) for t in init]) for d in ("cpu", DEV)]
+        opts = [AdamW(1e-2, state_bits=bits, global_clipnorm=clip) for _ in arenas]
+        for o, a in zip(opts, arenas):
+            o.bind(a)
+        for t in range(1, 13):
+            grad = torch.randn(arenas[0].numel, generator=g) * 10.0 ** (t % 5 - 3)
+            for o, a in zip(opts, arenas):
+                a.grad.copy_(grad)
+                o.step(grad_scale=0.3)
+            for k, v in opts[0].state_tensors().items():
+                assert torch.equal(v, opts[1].state_tensors()[k].cpu()), (k, t)
