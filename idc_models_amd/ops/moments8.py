@@ -47,7 +47,8 @@ def encode(x: torch.Tensor, mantissa: int, bits16: Optional[torch.Tensor] = None
     if mantissa == ROOT_BITS:
         code = torch.maximum(code, (a.view(-1) > 0).int())
     else:
-        code = code | ((x < 0) & ~bad.repeat_interleave(BLOCK)).int() << 7
+        # the sign bit, of zeros too, as the kernel keeps it: a value that rounded to -0 is code 0x80
+        code = code | (torch.signbit(x) & ~bad.repeat_interleave(BLOCK)).int() << 7
     return code.to(torch.uint8), scale.to(torch.uint8)
 
 

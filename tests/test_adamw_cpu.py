@@ -168,3 +168,19 @@ def test_memory_at_held_addresses():
     assert not held.moved()
     net.to(torch.float64)
     assert held.moved()
+
+
+def test_zeros_keep_their_sign():
+    """A first moment of -0.0 is code 0x80, as the kernel writes it, and stays so when it is decoded and encoded; a
+    block that is not finite holds no signs."""
+    x = torch.ones(128)
+    x[1], x[2], x[3], x[4], x[70] = -0.0, 0.0, -1e-30, -1.0, -2.0
+    codes, scales = moments8.encode(x, moments8.M_BITS)
+    assert codes[:5].tolist() == [codes[0], 0x80, 0, 0x80, int(codes[0]) | 0x80]
+    m = moments8.decode(codes, scales, moments8.M_BITS)
+    assert torch.signbit(m).nonzero().flatten().tolist() == [1, 3, 4, 70]
+    again, _ = moments8.encode(m, moments8.M_BITS)
+    assert torch.equal(again, codes)
+    x[100] = float("nan")
+    codes, _ = moments8.encode(x, moments8.M_BITS)
+    assert bool((codes[64:] == 0).all()) and codes[1] == 0x80

@@ -231,3 +231,30 @@ def test_cpu_and_gpu_states_are_the_same_bits_when_clipped(bits, clip):
                 o.step(grad_scale=0.3)
             for k, v in opts[0].state_tensors().items():
                 assert torch.equal(v, opts[1].state_tensors()[k].cpu()), (k, t)
+
+
+def test_cpu_and_gpu_codes_of_negative_zeros():
+    """Gradients of -0.0 (as a masked backward leaves) that meet first moments which have rounded to -0: the CPU's
+    codes, signs of zeros among them, are the GPU's."""
+    from idc_models_amd.engine import AdamW, ParamArena
+    arenas = [ParamArena([torch.nn.Parameter(torch.ones(64 * 6, device=d))]) for d in ("cpu", DEV)]
+    opts = [AdamW(1e-2, state_bits=8) for _ in arenas]
+    for o, a in zip(opts, arenas):
+        o.bind(a)
+    first = torch.full((384,), -1e-12)
+    first[::64] = 1.0  # the others' values are far below a unit of their block
+    first[320:] = -0.0
+    zeros = torch.where(torch.arange(384) % 3 == 0, 0.0, -0.0)
+    seen = 0
+    for grad in (first, zeros, zeros, -zeros, zeros):
+        for o, a in zip(opts, arenas):
+            a.grad.copy_(grad)
+            o.step()
+        for k, v in opts[0].state_tensors().items():
+            assert torch.equal(v, opts[1].state_tensors()[k].cpu()), k
+        seen += int((opts[0].m == 0x80).sum())
+    assert seen > 300
+    # a checkpoint of the other width keeps them as well
+    m, v = opts[1].moments()
+    opts[0].load_slots({"m": m.cpu(), "v": v.cpu(), "step": opts[0].steps})
+    assert torch.equal(opts[0].m, opts[1].m.cpu()) and torch.equal(opts[0].scales, opts[1].scales.cpu())
