@@ -97,7 +97,7 @@ enum OpKind : int {
   // a whole DenseNet dense block in inference mode (dense_infer.hip): payload DenseInferArgs
   OP_DENSE_INFER = 32,
   // multi-tensor AdamW step (adamw.hip): payload AdamwArgs, i[0] state bits, i[1] bf16 gradients, f[0]
-  // learning rate, f[1] weight decay; p[0] and i[2]: the piece table and its length again
+  // learning rate, f[1] its product with the weight decay; p[0] and i[2]: the piece table and its length again
   OP_ADAMW = 33,
   // partial sums of the squared gradients (adamw.hip): p[0] device OptChunk[i[0]], p[1] partials,
   // i[1] bf16 gradients
@@ -645,8 +645,8 @@ class Plan {
         break;
       case OP_ADAMW: {
         AdamwArgs a = as<AdamwArgs>(op);
-        a.lr = op.f[0];  // (set_float changes it)
-        a.lr_wd = op.f[0] * op.f[1];
+        a.lr = op.f[0];  // (set_float changes both: the product is rounded once, from doubles, by the caller)
+        a.lr_wd = op.f[1];
         check(adamw(a, op.i[0], op.i[1], st), "adamw");
         break;
       }

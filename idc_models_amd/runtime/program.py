@@ -168,6 +168,7 @@ class FusedProgram:
             b.step_flag = b._stats_floats(4).view(torch.int32)
         # optimizer segment
         self.nonfinite_status = None
+        self._weight_decay = None  # of a fused AdamW update
         if training and model.arena.params:
             opt = model.optimizer
             self.host_optimizer = not opt.native_step
@@ -358,6 +359,7 @@ class FusedProgram:
         from ..ops import optim
         # the plan holds addresses only: the optimizer may be bound to another model while it lives
         t, st = self._opt_keep = opt.table, opt.state
+        self._weight_decay = opt.weight_decay
         a = optim.set_adamw_args(nat.AdamwArgs.from_buffer_copy(st._args), t, st, opt.learning_rate, opt.beta_1,
                                  opt.beta_2, opt.epsilon, opt.weight_decay, grad_scale, opt.clip_norm, skip, hostflag)
         bf16 = int(t.grad_dtype == torch.bfloat16)
@@ -365,7 +367,7 @@ class FusedProgram:
             b.emit(nat.OP_GRAD_NORM, ints=(t.nchunks, bf16), ptrs=(a.chunks, a.partials))
         # the piece table and its length also as operands: a grouped program checks its pointers there
         b.emit(nat.OP_ADAMW, payload=a, ints=(st.bits, bf16, t.nchunks),
-               floats=(opt.learning_rate, opt.weight_decay), ptrs=(a.chunks,))
+               floats=(opt.learning_rate, opt.learning_rate * opt.weight_decay), ptrs=(a.chunks,))
 
     # ------------------------------------------------------------------ execution
     def _sh(self):
@@ -480,6 +482,8 @@ class FusedProgram:
     def set_lr(self, lr: float):
         if self.opt_index is not None:
             self.plan.set_float(self.opt_index, 0, float(lr))  # RMSprop's and AdamW's first float
+            if self._weight_decay is not None:
+                self.plan.set_float(self.opt_index, 1, float(lr) * self._weight_decay)
             self.plan.clear_graphs()
             self.graphs = {}
             self._bwd_graphs = None

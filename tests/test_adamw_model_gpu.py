@@ -258,3 +258,32 @@ def test_cpu_and_gpu_codes_of_negative_zeros():
     m, v = opts[1].moments()
     opts[0].load_slots({"m": m.cpu(), "v": v.cpu(), "step": opts[0].steps})
     assert torch.equal(opts[0].m, opts[1].m.cpu()) and torch.equal(opts[0].scales, opts[1].scales.cpu())
+
+
+@pytest.mark.parametrize("bits,clip", [(32, None), (8, 0.1)])
+def test_fused_update_is_adamw_(bits, clip):
+    """The fused program's update gives the bits of adamw_ on the same gradients, also after set_lr; learning rates
+    and decays whose product in fp32 is not the rounded product."""
+    import numpy as np
+    from idc_models_amd.engine import AdamW
+    from idc_models_amd.ops import optim
+    lr, wd = 1e-3, 0.004
+    opt = AdamW(lr, weight_decay=wd, global_clipnorm=clip, state_bits=bits)
+    m = model(opt, "mobilenetv2")
+    x, y = batch()
+    for t in range(4):
+        assert np.float32(lr) * np.float32(wd) != np.float32(lr * wd)
+        w = m.arena.data.clone()
+        state = {k: v.clone() for k, v in opt.state_tensors().items()}
+        m.impl.train_step(x, y)
+        torch.cuda.synchronize()
+        table = optim.TensorTable([m.arena.grad], [w])
+        st = optim.AdamWState(table, bits=bits)
+        for k, v in st.tensors().items():
+            v.copy_(state[k])
+        optim.adamw_(table, st, lr, weight_decay=wd, clip_norm=clip or 0.0)
+        assert torch.equal(w, m.arena.data)
+        assert all(torch.equal(v, opt.state_tensors()[k]) for k, v in st.tensors().items())
+        if t == 1:
+            lr = 3e-4
+            next(iter(m.impl.progs.values())).set_lr(lr)
