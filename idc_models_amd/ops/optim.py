@@ -180,7 +180,8 @@ class TensorTable:
 
 
 class AdamWState:
-    """Moments and step counter of an AdamW step over a table's tensors.
+    """Moments and step counter of an AdamW step over a table's tensors, or over those of another table of
+    tensors of the same sizes in the same order.
 
     ``bits=32``: ``m`` and ``v`` are fp32, ``table.numel`` long.  ``bits=8``: codes of the first moment
     and of the root of the second (uint8), and ``scales``, two bytes for 64 of them: 2.03 bytes a
@@ -192,7 +193,7 @@ class AdamWState:
             raise ValueError(f"AdamW states have 8 or 32 bits, not {bits}")
         if table.params is None:
             raise ValueError("the table has no params")
-        self.bits, self.numel, self.device = bits, table.numel, table.device
+        self.bits, self.numel, self.device, self.sizes = bits, table.numel, table.device, table.sizes
         dtype = torch.uint8 if bits == 8 else torch.float32
         room = max(self.numel, nat.OPT_BLOCK)  # a table of empty tensors still has a state
         self.m = torch.zeros(room, dtype=dtype, device=self.device)[:self.numel]
@@ -324,7 +325,8 @@ def adamw_(table: TensorTable, state: AdamWState, lr: float, beta_1: float = 0.9
         raise ValueError(f"grad_scale has to be finite: {grad_scale}")
     if table.params is None:
         raise ValueError("the table has no params")
-    if state.numel != table.numel or state.device != table.device:
+    # every tensor's moments lie at its place (the first comparison is what a program meets that keeps its table)
+    if (state.sizes is not table.sizes and state.sizes != table.sizes) or state.device != table.device:
         raise ValueError("the state was made for another table")
     if table._leaves.moved():
         raise ValueError("a weight has other storage than when the table was made")

@@ -184,3 +184,16 @@ def test_zeros_keep_their_sign():
     x[100] = float("nan")
     codes, _ = moments8.encode(x, moments8.M_BITS)
     assert bool((codes[64:] == 0).all()) and codes[1] == 0x80
+
+
+def test_state_of_other_tensors_is_refused():
+    """Tables of [100, 30] and [30, 100] have states of one length, with other tensors' moments in it."""
+    from types import SimpleNamespace
+    dev = torch.device("cpu")
+    table = lambda sizes: SimpleNamespace(params=[], sizes=list(sizes), numel=192, device=dev, _leaves=optim._Held([]))
+    state = SimpleNamespace(sizes=[100, 30], numel=192, device=dev)
+    for sizes in ([30, 100], [100, 31], [128, 64], [192], [100, 30, 0]):
+        with pytest.raises(ValueError, match="another table"):
+            optim.adamw_(table(sizes), state, 1e-3)
+    with pytest.raises(ValueError, match="skip"):  # the same sizes: on to the next check
+        optim.adamw_(table([100, 30]), state, 1e-3, skip=torch.zeros(1))

@@ -530,3 +530,17 @@ def test_weights_whose_storage_is_replaced(bits):
     optim.adamw_(table, st, **HYPER)
     torch.cuda.synchronize()
     assert all(bool((o == 7.0).all()) for o in others) and float(w.abs().max()) == 0.0
+
+
+def test_state_and_tables_of_the_same_length():
+    """A state goes with its tensors' sizes: tables in another order are refused, a second table of the same tensors
+    is fine."""
+    from idc_models_amd.ops import optim
+    ps, gs = [rand(n, seed=n).to(DEV) for n in (100, 30)], [rand(n, seed=n + 1).to(DEV) for n in (100, 30)]
+    st = optim.AdamWState(optim.TensorTable(gs, ps))
+    before = [p.clone() for p in ps]
+    with pytest.raises(ValueError, match="another table"):
+        optim.adamw_(optim.TensorTable(gs[::-1], ps[::-1]), st, **HYPER)
+    assert int(st.step[0]) == 0 and all(torch.equal(p, b) for p, b in zip(ps, before))
+    gs = [g.clone() for g in gs]
+    check_step(ps, gs, optim.TensorTable(gs, ps), st, [True, True])
