@@ -70,6 +70,12 @@ class _Held:
         # one call into torch: 0.1 us for a tensor, 16 for 600 (data_ptr() in Python: 0.13 and 24)
         return bool(self.every) and not torch._C._tensors_data_ptrs_at_indices_equal(self.tensors, self.at, self.every)
 
+    def changed(self) -> None:
+        """Tells autograd that a kernel has written to the tensors: a backward pass through a graph that saved
+        them raises, as after any operation in place."""
+        if self.every:
+            torch.autograd.graph.increment_version(self.tensors)
+
 
 def chunk_size(sizes: Sequence[int]) -> int:
     """Elements of a full piece of a table (csrc/kernels/adamw.h)."""
@@ -319,7 +325,10 @@ def adamw_(table: TensorTable, state: AdamWState, lr: float, beta_1: float = 0.9
     ``clip_norm`` > 0 scales g down to that global norm (one launch more for all but small tables, nothing
     is read back; a norm that is not finite makes every gradient NaN).  ``skip``: an int32 tensor on the
     device; if its first word is not zero the call changes nothing.  The numbers are arguments of the
-    launch: a captured call keeps those it was captured with, and counts its steps on the device."""
+    launch: a captured call keeps those it was captured with, and counts its steps on the device.
+
+    Autograd sees the change of weights that are Parameters or require a gradient (a replayed graph's changes
+    it does not see): a second backward pass through a graph that saved them raises."""
     check_adamw(lr, beta_1, beta_2, epsilon, weight_decay, clip_norm)
     if not abs(grad_scale) <= _MAX:
         raise ValueError(f"grad_scale has to be finite: {grad_scale}")
@@ -340,6 +349,7 @@ def adamw_(table: TensorTable, state: AdamWState, lr: float, beta_1: float = 0.9
         if a.partials:
             ext.grad_norm(a.chunks, table.nchunks, table._bf16, a.partials, 0, stream)
         ext.adamw(ctypes.addressof(a), state.bits, table._bf16, stream)
+    table._leaves.changed()
 
 
 def global_norm(table: TensorTable) -> torch.Tensor:

@@ -197,3 +197,17 @@ def test_state_of_other_tensors_is_refused():
             optim.adamw_(table(sizes), state, 1e-3)
     with pytest.raises(ValueError, match="skip"):  # the same sizes: on to the next check
         optim.adamw_(table([100, 30]), state, 1e-3, skip=torch.zeros(1))
+
+
+def test_autograd_is_told_of_changes():
+    w, x = torch.nn.Parameter(torch.ones(5)), torch.ones(5, requires_grad=True)
+    with torch.inference_mode():
+        other = torch.zeros(3)  # has no version
+    held = optim._Held([w, other])
+    y = (w * x).sum()
+    y.backward(retain_graph=True)
+    held.changed()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    (w * x).sum().backward()
+    optim._Held([]).changed()

@@ -544,3 +544,44 @@ def test_state_and_tables_of_the_same_length():
     assert int(st.step[0]) == 0 and all(torch.equal(p, b) for p, b in zip(ps, before))
     gs = [g.clone() for g in gs]
     check_step(ps, gs, optim.TensorTable(gs, ps), st, [True, True])
+
+
+def test_a_second_backward_after_a_step_raises():
+    """As after torch's own optimizers: the graph saved the weights that the step has changed.  A refused
+    call changes nothing, so the graph stays good."""
+    from idc_models_amd.ops import optim
+    lin = torch.nn.Linear(70, 33).to(DEV)
+    x = rand(8, 70, seed=1).to(DEV).requires_grad_()
+    lin(x).square().sum().backward()
+    table = optim.TensorTable([p.grad for p in lin.parameters()], list(lin.parameters()))
+    st = optim.AdamWState(table)
+    y = lin(x).square().sum()
+    y.backward(retain_graph=True)
+    with pytest.raises(ValueError):
+        optim.adamw_(table, st, -1.0)
+    y.backward(retain_graph=True)
+    optim.adamw_(table, st, **HYPER)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    for _ in range(2):  # steps whose graphs are new go on
+        for p in lin.parameters():
+            p.grad.zero_()
+        lin(x).square().sum().backward()
+        check_step([p for p in lin.parameters()], [p.grad for p in lin.parameters()], table, st, [True, True])
+
+
+def test_version_of_captured_steps():
+    """A step over Parameters can be captured; each eager call is one change for autograd."""
+    from idc_models_amd.ops import optim
+    p = torch.nn.Parameter(rand(500, seed=1).to(DEV))
+    g = rand(500, seed=2).to(DEV)
+    table = optim.TensorTable([g], [p])
+    st = optim.AdamWState(table)
+    v = p._version
+    optim.adamw_(table, st, **HYPER)
+    assert p._version > v
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        optim.adamw_(table, st, **HYPER)
+    for _ in range(3):
+        check_step([p], [g], table, st, [True], call=graph.replay)
