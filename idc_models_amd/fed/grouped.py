@@ -1,6 +1,6 @@
 """Client-batched local training: a rank's K federated clients advance in lockstep through ONE
 grouped program (``runtime/grouped.py``): every kernel launch of a step covers all K clients, each
-with its own weights, BatchNorm statistics, RMSprop slots, inputs and labels.
+with its own weights, BatchNorm statistics, optimizer slots, inputs and labels.
 
 Semantics are exactly those of training the clients one after another on one worker model
 (``FedAvgProcess._train_client``, TFF ``fed_model.py:207-229``): every client starts from the
@@ -8,8 +8,9 @@ server weights with a fresh client optimizer and fresh statistics shifts, and dr
 shuffled batches (its dataset's own seed and epoch counter).  Under ``IDC_DETERMINISTIC=1`` the
 per-client results are bitwise those of the sequential path (``tests/test_fed_gpu.py``).
 
-Eligibility (else the sequential path runs): fused backend on a GPU, one logit, and client datasets
-that are ``BatchedDataset`` s with ``drop_remainder`` and the same batch size and step count.
+Eligibility (else the sequential path runs): fused backend on a GPU, one logit, an optimizer that the
+program carries (RMSprop without momentum, AdamW), and client datasets that are ``BatchedDataset`` s with
+``drop_remainder`` and the same batch size and step count.
 """
 from __future__ import annotations
 
@@ -26,6 +27,10 @@ def eligible(datasets: Sequence, model) -> bool:
     if model.device.type != "cuda" or getattr(model.impl, "name", "") != "fused":
         return False
     if getattr(model.net, "num_outputs", 1) != 1 or not datasets:
+        return False
+    # the copies' weights are updated by the program alone: an optimizer that steps on the host (SGD, RMSprop
+    # with momentum) would never be called
+    if not model.optimizer.native_step:
         return False
     if not all(isinstance(d, BatchedDataset) and d.drop_remainder and d.repeat == 1 for d in datasets):
         return False

@@ -217,3 +217,19 @@ def test_clipped_gradients_take_one_quotient():
         norm = f(np.sqrt(np.square(grad.astype(np.float64)).sum())) * f(0.3)
         want = f(0.1) * ((grad * f(0.3)) * (f(0.7) / norm))
         assert want.dtype == f and (opt.m.numpy() == want).all(), seed
+
+
+def test_client_batching_needs_an_optimizer_that_the_program_carries():
+    """A grouped program updates its weights by itself: clients whose optimizer steps on the host train one after
+    another."""
+    from types import SimpleNamespace
+    from idc_models_amd.data import contiguous_clients, synthetic_dataset
+    from idc_models_amd.engine import SGD, RMSprop
+    from idc_models_amd.fed.grouped import eligible
+    sets = [c.batch(8, drop_remainder=True) for c in contiguous_clients(synthetic_dataset(32, (10, 10, 3), seed=2), 2, 16)]
+    model = lambda opt: SimpleNamespace(device=torch.device("cuda"), impl=SimpleNamespace(name="fused"),
+                                        net=SimpleNamespace(num_outputs=1), optimizer=opt)
+    for opt in (RMSprop(), AdamW(), AdamW(state_bits=8)):
+        assert eligible(sets, model(opt))
+    for opt in (SGD(0.1), SGD(0.1, momentum=0.9), RMSprop(momentum=0.9), RMSprop(centered=True)):
+        assert not eligible(sets, model(opt))

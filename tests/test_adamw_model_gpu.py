@@ -287,3 +287,27 @@ def test_fused_update_is_adamw_(bits, clip):
         if t == 1:
             lr = 3e-4
             next(iter(m.impl.progs.values())).set_lr(lr)
+
+
+def test_clients_with_a_host_optimizer_train(monkeypatch):
+    """SGD clients under client batching: the same round as one after another (they do not share a program, which
+    would leave their weights as they were)."""
+    from idc_models_amd.data import contiguous_clients, synthetic_dataset
+    from idc_models_amd.engine import SGD, Model
+    from idc_models_amd.fed import build_federated_averaging_process
+    from idc_models_amd.models import build_model
+    from idc_models_amd.parallel import OneDeviceStrategy
+    monkeypatch.setenv("IDC_DETERMINISTIC", "1")
+    base = build_model("vgg16", None, 1, seed=3)
+    ds = synthetic_dataset(2 * 32, (50, 50, 3), 2, seed=7)
+
+    def run(batching):
+        clients = [c.batch(16, True, 1000, True, seed=k) for k, c in enumerate(contiguous_clients(ds, 2, 32))]
+        proc = build_federated_averaging_process(lambda: Model(copy.deepcopy(base), OneDeviceStrategy(DEV)),
+                                                 lambda: SGD(0.05), backend="fused", client_batching=batching)
+        s0 = proc.initialize()
+        s1, _ = proc.next(s0, clients)
+        return [torch.cat([w.reshape(-1) for w in s.model.trainable]) for s in (s0, s1)]
+
+    (a0, a1), (b0, b1) = run(False), run(True)
+    assert torch.equal(a0, b0) and torch.equal(a1, b1) and not torch.equal(a0, a1)
