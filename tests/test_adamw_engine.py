@@ -233,3 +233,40 @@ def test_client_batching_needs_an_optimizer_that_the_program_carries():
         assert eligible(sets, model(opt))
     for opt in (SGD(0.1), SGD(0.1, momentum=0.9), RMSprop(momentum=0.9), RMSprop(centered=True)):
         assert not eligible(sets, model(opt))
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_secure_clients_keep_their_adamw_state(bits):
+    """Clients of a secure federated process share one model and optimizer, whose slots (moments, scales, step
+    counter) are swapped: after two rounds each has the bits of a client with an optimizer of its own."""
+    from idc_models_amd.data import shard_clients, synthetic_dataset
+    from idc_models_amd.fed import SecureFederatedProcess
+    ds = synthetic_dataset(48, (10, 10, 3), seed=3)
+    sets = lambda: [(s.take(18).batch(6, False), s.skip(18).batch(6, False)) for s in shard_clients(ds, 2)]
+
+    def make():
+        return tiny(AdamW(1e-2, global_clipnorm=0.5, state_bits=bits))
+
+    proc = SecureFederatedProcess(make, sets(), percent=1.0, mode="mask", epochs=2)
+    own = [make() for _ in range(2)]
+    for k, m in enumerate(own):
+        with torch.no_grad():
+            for t, w in zip(m.net.weights, proc.states[k].weights):
+                t.copy_(w)
+    data = sets()
+    for r in range(2):
+        for k, m in enumerate(own):
+            torch.manual_seed(10 * r + k)  # dropout
+            proc.client_fit(k)
+            torch.manual_seed(10 * r + k)
+            m.fit(data[k][0], epochs=2, validation_data=data[k][1], verbose=0)
+            assert all(torch.equal(a, b) for a, b in zip(proc.states[k].weights, m.net.weights))
+            slots = m.optimizer.state_tensors()
+            assert set(slots) == set(proc.states[k].opt_slots) and int(slots["step"][0]) == 6 * (r + 1)
+            assert all(torch.equal(v, proc.states[k].opt_slots[n]) for n, v in slots.items())
+        avg = proc.aggregate()  # both take the mean, with their own moments
+        for k, m in enumerate(own):
+            proc.states[k].weights = [a.detach().clone() for a in avg]
+            with torch.no_grad():
+                for t, a in zip(m.net.weights, avg):
+                    t.copy_(a)

@@ -585,3 +585,44 @@ def test_version_of_captured_steps():
         optim.adamw_(table, st, **HYPER)
     for _ in range(3):
         check_step([p], [g], table, st, [True], call=graph.replay)
+
+
+LARGE = {"2048-element pieces": ([2048 * 700 + 3, 2048 * 900, 77], 2048), "4096-element pieces": ([4096 * 700 + 3, 4096 * 400, 77], 4096),
+         "past the caches": ([4096 * 2800 + 3, 77], 4096)}  # (32 bits: from 1,366 pieces on; 8 bits: from 2,731)
+
+
+@pytest.mark.parametrize("sizes", LARGE, ids=lambda k: k.replace(" ", "-"))
+@pytest.mark.parametrize("grad_dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_every_kind_of_large_table(bits, grad_dtype, sizes):
+    """More pieces than workgroups: both piece sizes, cached and past the caches, either width and gradient type;
+    tensors of their own, and at addresses that vector accesses cannot use."""
+    sizes, chunk = LARGE[sizes]
+    for layout in ("own", "odd"):
+        params, grads, buf = make(sizes, layout, grad_dtype, seed=9)
+        decay = [i != 1 for i in range(len(sizes))]
+        table, st = start(params, grads, bits, 5, decay)
+        assert 1024 < table.nchunks < 8192 and table.chunk == chunk
+        assert (table.nchunks * chunk * (12 if bits == 8 else 24) >= 128 << 20) == (len(sizes) == 2)
+        check_step(params, grads, table, st, decay, 1.0, 1.0)
+        if buf is not None:
+            wb, gb, outside = buf
+            assert bool((wb[outside] == 7.0).all()) and bool((gb[outside] == 7.0).all())
+
+
+@pytest.mark.parametrize("grad_dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_global_norm_of_large_pieces(grad_dtype):
+    """Tables of 4096-element pieces; pieces of zeros and of values whose squares are no fp32 numbers among them."""
+    from idc_models_amd.ops.optim import TensorTable, global_norm
+    n = 4096 * 1100 + 2048 + 5  # its last pieces have 4096 and 2053 elements
+    for layout in ("own", "odd"):
+        _, grads, _ = make([n, 2048, 9], layout, grad_dtype, seed=7)
+        table = TensorTable(grads)
+        assert table.chunk == 4096 and table.nchunks == 1103
+        for value in (None, 0.0, 1e-30, 1e25):
+            if value is not None:
+                grads[0][:4096 * 8].view(8, 4096)[::2] = value
+            want = orc.norm(grads)
+            # one rounding to fp32; bf16: sums of 16 exact squares in fp32, 4 roundings deep, which the root halves
+            tol = orc.U if grad_dtype is torch.float32 else 3 * orc.U
+            assert abs(float(global_norm(table)) - want) <= (tol + 2.0 ** -40) * want
