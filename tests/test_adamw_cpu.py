@@ -158,9 +158,10 @@ def test_memory_at_held_addresses():
     p.data = torch.full((1000,), 5.0)
     assert held.moved()
     others = [torch.full((1000,), 7.0) for _ in range(20)]  # none of them gets the first storage
-    assert held.aliases[1].data_ptr() == at and bool((held.aliases[1] == 2.0).all())
+    first = torch.empty(0).set_(held.memory[1])
+    assert first.data_ptr() == at and bool((first == 2.0).all()) and first.numel() == 1000
     assert all(t.data_ptr() != at for t in others)
-    p.data = held.aliases[1]
+    p.data = first
     assert not held.moved()
     net = torch.nn.Linear(3, 4)
     held = optim._Held(list(net.parameters()))
@@ -190,7 +191,7 @@ def test_state_of_other_tensors_is_refused():
     """Tables of [100, 30] and [30, 100] have states of one length, with other tensors' moments in it."""
     from types import SimpleNamespace
     dev = torch.device("cpu")
-    table = lambda sizes: SimpleNamespace(params=[], sizes=list(sizes), numel=192, device=dev, _leaves=optim._Held([]))
+    table = lambda sizes: SimpleNamespace(params=[], sizes=list(sizes), numel=192, device=dev, _leaves=None)
     state = SimpleNamespace(sizes=[100, 30], numel=192, device=dev)
     for sizes in ([30, 100], [100, 31], [128, 64], [192], [100, 30, 0]):
         with pytest.raises(ValueError, match="another table"):
