@@ -1,7 +1,7 @@
 """Fused optimizer entry points (native HIP kernels over flat fp32 arenas or many tensors).
 
 ``rmsprop_`` updates one flat arena.  The AdamW step and the global norm of the gradients take a
-``TensorTable``, which describes any number of tensors once, so that a call is one or two launches:
+``TensorTable``, which describes any number of tensors once, so that a call is one to three launches:
 
     table = TensorTable(grads, params, decay=[p.dim() > 1 for p in params])
     state = AdamWState(table, bits=8)
@@ -318,7 +318,7 @@ def set_adamw_args(a: "nat.AdamwArgs", table: TensorTable, state: AdamWState, lr
 def adamw_(table: TensorTable, state: AdamWState, lr: float, beta_1: float = 0.9, beta_2: float = 0.999,
            epsilon: float = 1e-7, weight_decay: float = 0.004, grad_scale: float = 1.0, clip_norm: float = 0.0,
            skip: Optional[torch.Tensor] = None) -> None:
-    """One Keras AdamW step over the table's tensors, in place, in one launch:
+    """One Keras AdamW step over the table's tensors, in place, in one launch (two from 33.5 million weights on):
 
         t += 1;  g = grad_scale * grad;  m = beta_1*m + (1-beta_1)*g;  v = beta_2*v + (1-beta_2)*g^2
         w -= lr*weight_decay*w + lr*sqrt(1-beta_2^t)/(1-beta_1^t) * m/(sqrt(v)+epsilon)
