@@ -110,8 +110,9 @@ class TensorTable:
     The addresses are read here once: gradients have to be accumulated in place afterwards, as an
     arena's are, and weights have to keep their storage.  Where it is replaced (``p.data = x``,
     ``Module.to``, ``Model.compile``, which moves a model's weights into an arena), a new table is needed: ``adamw_``
-    refuses weights that are Parameters or require a gradient, ``check`` any tensor.  The table keeps the memory
-    alive.  A weight and its gradient have the same shape and the same order of axes in memory, without
+    refuses weights that are Parameters or require a gradient, ``check`` any tensor.  The table keeps the first
+    storage alive, but resizing a listed tensor in place frees its memory all the same: not before the table's last
+    call.  A weight and its gradient have the same shape and the same order of axes in memory, without
     gaps.  Empty tensors are fine.  ``decay``: which weights decay (default: all)."""
 
     def __init__(self, grads: Sequence[torch.Tensor], params: Optional[Sequence[torch.Tensor]] = None,
